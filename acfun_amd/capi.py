@@ -78,6 +78,17 @@ SIGNATURES = {
     "acfun_dev_maxpool": (_i, [_p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p]),
     "acfun_dev_fc": (_i, [_p, _i, _i, _p, _p, _i, _p, _i, _p]),
     "acfun_dev_softmax": (_i, [_p, _i, _i, _p, _p]),
+    "acfun_mxfp4_code_bytes": (_sz, [_i, _i]),
+    "acfun_mxfp4_scale_bytes": (_sz, [_i, _i]),
+    "acfun_dev_quantize_mxfp4": (_i, [_p, _i, _i, _i, _i, _p, _p, _p]),
+    "acfun_dev_dequantize_mxfp4": (_i, [_p, _p, _i, _i, _p, _i, _p]),
+    "acfun_dev_gemm_mxfp4": (_i, [_i, _i, _i, _p, _p, _p, _p, _p, _i, _p, _i, _p]),
+    "acfun_dev_fc_mxfp4": (_i, [_p, _i, _i, _i, _p, _p, _p, _i, _p, _i, _p]),
+    "acfun_quantize_weights_mxfp4": (None, [_p, _i, _i, _p, _p]),
+    "acfun_fc_mxfp4": (None, [_p, _i, _i, _p, _p, _p, _i, _p, _i]),
+    "acfun_dev_norm": (_i, [_p, _i, _i, _i, _i, _p, _p, _f, _p, _p]),
+    "acfun_dev_norm_residual": (_i, [_p, _p, _i, _i, _i, _i, _p, _p, _p, _i, _f, _p, _p, _f, _p,
+                                     _p, _p]),
     "acfun_model_load_ex": (_p, [_s, _i]),
     "acfun_model_infer_batch": (_i, [_p, _i, _p, _p]),
     "acfun_dev_model_infer_batch": (_i, [_p, _i, _p, _p, _p]),

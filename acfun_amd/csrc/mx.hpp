@@ -1,0 +1,78 @@
+// mx.hpp -- MXFP4 operands (microscaled 4-bit floating point) and the element
+// types of the float tensors of the transformer-layer entry points.
+//
+// A block is 32 consecutive k of one row: 32 codes of 4 bits (e2m1: sign, then
+// 0, 0.5, 1, 1.5, 2, 3, 4, 6) and one scale byte (e8m0: 2^(byte - 127); 255 = NaN).
+// With a = max|x| of the block, byte = max(floor(log2 a) - 2, -127) + 127, and a
+// code is x / 2^(byte - 127) rounded to the nearest value, halves to the even
+// code, at most 6.  A NaN or an infinity in a block gives byte 255.
+//
+// Both arrays are laid out as the scaled MFMA reads them.  Codes: tiles of 16
+// rows x 128 k, 1024 bytes each, row tiles outermost; the 16 bytes of block j
+// (of 4) and row r of a tile are its number 16 j + r, which is the lane that
+// feeds them to v_mfma_scale_f32_16x16x128; k even is the low half of a byte.
+// A tile is one contiguous kilobyte: one wave's 16-byte loads, and one
+// contiguous read from LDS.  Scale bytes: tiles of 16 rows x 512 k, 256 bytes
+// each; byte 4 (16 j + r) + s belongs to block j of the tile's s-th 128 k, so
+// that a lane's dword holds its scales for four MFMAs and op_sel picks one.
+// Rows are padded to 16, codes to 128 k and scales to 512 k; the quantizer
+// writes zeros there.
+#pragma once
+#include "rt.hpp"
+
+namespace acfun {
+
+// Element types of float tensors (ACFUN_F32, ACFUN_BF16, ACFUN_F16).
+inline bool type_ok(int t) { return t >= 0 && t <= 2; }
+inline size_t type_size(int t) { return t == 0 ? 4 : 2; }
+// Calls f with a value of the C++ type.
+template <class F>
+auto with_type(int t, F f) {
+    return t == 0 ? f(0.f) : t == 1 ? f((__bf16)0.f) : f((_Float16)0.f);
+}
+
+__host__ __device__ inline long long mx_row_tiles(int rows) { return ((long long)rows + 15) / 16; }
+__host__ __device__ inline int mx_k_tiles(int K) { return (int)(((long long)K + 127) / 128); }
+__host__ __device__ inline int mx_scale_tiles(int K) { return (int)(((long long)K + 511) / 512); }
+inline size_t mx_code_bytes(int rows, int K) { return (size_t)mx_row_tiles(rows) * mx_k_tiles(K) * 1024; }
+inline size_t mx_scale_bytes(int rows, int K) { return (size_t)mx_row_tiles(rows) * mx_scale_tiles(K) * 256; }
+
+// A block's scale byte from the bits of max|x| as fp32 (the largest of the
+// values' bit patterns without sign: NaN and infinity are the largest).
+__device__ __forceinline__ unsigned mx_scale_byte(unsigned amax) {
+    const unsigned e = amax >> 23;
+    return e == 255 ? 255u : (e > 2 ? e - 2 : 0u);
+}
+// 2^(byte - 127); the hardware's conversions read the exponent of this.
+__device__ __forceinline__ float mx_scale_float(unsigned byte) {
+    return __uint_as_float(byte ? byte << 23 : 0x400000u);
+}
+
+// k_mx.hip
+bool mx_quantize(const void* x, int type, int rows, int K, int trans, uint8_t* codes, uint8_t* scales,
+                 hipStream_t s);
+bool mx_dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int K, void* x, int type,
+                   hipStream_t s);
+// k_mxmm.hip: C[M,N] = act(A B^T + bias), A and B in 4 bits.
+bool mx_gemm(int M, int N, int K, const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs,
+             void* C, int type, const float* bias, int act, hipStream_t s);
+// The same with float rows quantized in the call.
+bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_t* Bs, const float* bias,
+           int N, void* C, int act, hipStream_t s);
+
+// k_norm.hip
+struct NormArgs {
+    const void *y, *x;              // y: the block's output (null: h = norm(x) alone)
+    int rows, cols, layer;          // layer: subtract the mean
+    const float *post_w, *post_b;   // norm of y
+    const void* gate;               // [ceil(rows / gate_group)][cols], null: 1
+    int gate_group;
+    float res_scale;
+    const float *pre_w, *pre_b;     // norm of the sum
+    float eps;
+    void *x_out, *h;                // h null: no norm of the sum
+};
+bool norm_rows(const NormArgs& a, int type, hipStream_t s);
+constexpr int kNormMaxCols = 32768;
+
+}  // namespace acfun

@@ -245,6 +245,81 @@ int acfun_dev_fc(const float* input, int N, int Cin, const float* weight, const 
                  int Cout, float* output, int act, void* stream);
 int acfun_dev_softmax(const float* input, int rows, int cols, float* output, void* stream);
 
+/* ===================== new: transformer layers ===================== */
+
+/* Element types of the float tensors (`type`) of the calls below.  Parameters
+ * (bias, norm weights) are fp32 whatever the type.  Sums and statistics are
+ * held in fp32 and a result is rounded to its type once, when it is stored.
+ * The acfun_dev_* calls take device pointers and a stream as above; they return
+ * 0, or -1 with acfun_last_error() and nothing queued: on a negative size, an
+ * unknown type or code, a NULL or misaligned pointer.  An empty output is 0. */
+#define ACFUN_F32 0
+#define ACFUN_BF16 1
+#define ACFUN_F16 2
+
+/* Microscaled 4-bit floating point (MXFP4): 32 consecutive k of a row share
+ * one scale 2^e, e = max(floor(log2 max|x|) - 2, -127), kept as the byte
+ * e + 127; each value is the 4-bit code of the nearest of 0, 0.5, 1, 1.5, 2, 3,
+ * 4, 6 (with a sign) to x / 2^e, halves to the even code, at most 6.  A block
+ * with a NaN or an infinity has scale byte 255 and stands for NaN.
+ *
+ * An operand of `rows` rows is two arrays, each aligned to 16 bytes, in the
+ * order the matrix unit reads them (rows padded to 16, K as below, with zeros):
+ *   codes   tiles of 16 rows x 128 k, row tiles outermost, 1024 bytes each: byte
+ *           (16 j + r) * 16 + i of a tile holds k = 32 j + 2 i of row r in its low
+ *           half and k + 1 in its high half;
+ *   scales  tiles of 16 rows x 512 k, row tiles outermost, 256 bytes each: byte
+ *           4 (16 j + r) + s is that of row r, k = 128 s + 32 j .. + 31.
+ * The sizes of the arrays in bytes (0 for an empty operand): */
+size_t acfun_mxfp4_code_bytes(int rows, int K);
+size_t acfun_mxfp4_scale_bytes(int rows, int K);
+
+/* x [rows, K] (trans 0) or [K, rows] (trans 1: weights as acfun_fc takes them,
+ * rows = Cout) -> an operand; blocks run along K either way. */
+int acfun_dev_quantize_mxfp4(const void* x, int type, int rows, int K, int trans, uint8_t* codes,
+                             uint8_t* scales, void* stream);
+/* The values an operand stands for, as x [rows, K]. */
+int acfun_dev_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, int rows, int K, void* x,
+                               int type, void* stream);
+/* C[M,N] = A * B^T (+ bias[n], NULL = none; ReLU if act), A an operand of M rows,
+ * B of N rows; C of `type`.  K = 0 gives the bias alone. */
+int acfun_dev_gemm_mxfp4(int M, int N, int K, const uint8_t* A, const uint8_t* a_scales,
+                         const uint8_t* B, const uint8_t* b_scales, void* C, int type,
+                         const float* bias, int act, void* stream);
+/* A fully connected layer with weights held in MXFP4 (an operand of Cout rows):
+ * input [N, Cin] is quantized as acfun_dev_quantize_mxfp4 does and multiplied;
+ * output [N, Cout].  Input and output are of `type`. */
+int acfun_dev_fc_mxfp4(const void* input, int type, int N, int Cin, const uint8_t* weight,
+                       const uint8_t* wscale, const float* bias, int Cout, void* output, int act,
+                       void* stream);
+/* The same on host or device pointers, synchronous, fp32: weights w [K, N] into an
+ * operand of N rows, and the layer. */
+void acfun_quantize_weights_mxfp4(const float* w, int K, int N, uint8_t* codes, uint8_t* scales);
+void acfun_fc_mxfp4(const float* input, int N, int Cin, const uint8_t* weight, const uint8_t* wscale,
+                    const float* bias, int Cout, float* output, int act);
+
+/* Norms of rows (at most 32768 columns):
+ *   ACFUN_RMSNORM    norm(v) = v / sqrt(mean(v^2) + eps) * weight + bias
+ *   ACFUN_LAYERNORM  norm(v) = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias
+ * with weight and bias [cols], NULL meaning 1 and 0. */
+#define ACFUN_RMSNORM 0
+#define ACFUN_LAYERNORM 1
+
+/* Before a block: h = norm(x).  h may be x. */
+int acfun_dev_norm(const void* x, int type, int rows, int cols, int kind, const float* weight,
+                   const float* bias, float eps, void* h, void* stream);
+/* After a block with output y, in one pass:
+ *   x_out = res_scale * x + gate * norm(y; post_w, post_b)
+ *   h     = norm(x_out; pre_w, pre_b), the next block's input (NULL: not wanted)
+ * gate is [ceil(rows / gate_group), cols] of `type`, row r taking its row
+ * r / gate_group (1: a gate for each row, rows: one for all), NULL meaning 1.
+ * h is taken from the sum before x_out is rounded.  x_out may be x or y, and h
+ * may be y or x, but h and x_out are different buffers. */
+int acfun_dev_norm_residual(const void* y, const void* x, int type, int rows, int cols, int kind,
+                            const float* post_w, const float* post_b, const void* gate,
+                            int gate_group, float res_scale, const float* pre_w,
+                            const float* pre_b, float eps, void* x_out, void* h, void* stream);
+
 /* acfun_model_load with options: flags & 1 quantizes every dense conv (type 1)
  * to int8 at load (per-output-channel weights, acfun_quantize_weights rule) and
  * runs it through the acfun_conv2d_int8 rules; other layers stay fp32.  The
