@@ -31,6 +31,46 @@ auto with_type(int t, F f) {
     return t == 0 ? f(0.f) : t == 1 ? f((__bf16)0.f) : f((_Float16)0.f);
 }
 
+// Eight values, or 16 bytes, of a tensor from any element boundary: global loads and
+// stores need no more alignment than an element's.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f8u __attribute__((ext_vector_type(8), aligned(4)));
+typedef __bf16 b8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
+template <class T, int N> struct VecOf;
+template <> struct VecOf<float, 4> { typedef f4u type; };
+template <> struct VecOf<float, 8> { typedef f8u type; };
+template <> struct VecOf<__bf16, 8> { typedef b8u type; };
+template <> struct VecOf<_Float16, 8> { typedef h8u type; };
+// The first `left` of N values from p; `fill` for the others, which are not read.
+template <class T, int N>
+__device__ __forceinline__ typename VecOf<T, N>::type load_vec(const T* p, int left, float fill = 0.f) {
+    typename VecOf<T, N>::type v;
+    if (left >= N) return *(const typename VecOf<T, N>::type*)p;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = e < left ? p[e] : (T)fill;
+    return v;
+}
+template <class T, int N>
+__device__ __forceinline__ void store_vec(T* p, int left, const float (&v)[N]) {
+    if (left >= N) {
+        typename VecOf<T, N>::type o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = (T)v[e];
+        *(typename VecOf<T, N>::type*)p = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < left) p[e] = (T)v[e];
+    }
+}
+// Lane permutations: xor 1 and xor 2 within four lanes, the mirror of eight and of sixteen.
+template <int CTRL>
+__device__ __forceinline__ unsigned lane_perm(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;
+
 __host__ __device__ inline long long mx_row_tiles(int rows) { return ((long long)rows + 15) / 16; }
 __host__ __device__ inline int mx_k_tiles(int K) { return (int)(((long long)K + 127) / 128); }
 __host__ __device__ inline int mx_scale_tiles(int K) { return (int)(((long long)K + 511) / 512); }
