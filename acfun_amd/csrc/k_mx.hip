@@ -11,18 +11,6 @@ namespace {
 
 typedef unsigned u4v __attribute__((ext_vector_type(4)));
 
-// Eight values -> eight codes.
-__device__ __forceinline__ unsigned codes8(const float* v, float scale) {
-    unsigned r = 0;
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], scale, 0);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], scale, 1);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], scale, 2);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], scale, 3);
-    return r;
-}
-__device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
-__device__ __forceinline__ unsigned bits_abs(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
 // Rows along K.  A workgroup: one scale tile, 16 rows x 512 k.  Thread (r, j, p) has
 // the values 8 p .. 8 p + 7 of block j of row r of each of the four 128 k, so 16
 // threads read 128 consecutive k of a row, four of them share a block, and a wave
@@ -45,17 +33,11 @@ __global__ __launch_bounds__(256) void k_mx_quant(const T* __restrict__ x, int r
     unsigned bytes = 0;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        float f[8];
-        unsigned top = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (float)v[s][e], top = umax(top, bits_abs(f[e]));
-        top = umax(top, lane_perm<kXor1>(top));
-        top = umax(top, lane_perm<kXor2>(top));
-        const unsigned byte = mx_scale_byte(top);
+        unsigned byte;
+        const unsigned c = mx_codes_of4(v[s], byte);
         bytes |= byte << (8 * s);
         if (4 * b + s < kt)
-            ((unsigned*)codes)[(((size_t)rt * kt + 4 * b + s) * 64 + lane) * 4 + p] =
-                codes8(f, mx_scale_float(byte == 255 ? 0 : byte));
+            ((unsigned*)codes)[(((size_t)rt * kt + 4 * b + s) * 64 + lane) * 4 + p] = c;
     }
     if (p == 0) ((unsigned*)scales)[((size_t)rt * st + b) * 64 + lane] = bytes;
 }
@@ -88,7 +70,7 @@ __global__ __launch_bounds__(256) void k_mx_quant_t(const T* __restrict__ x, int
     if (tile && 4 * b + s < kt) {
         u4v c;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) c[q] = codes8(v + 8 * q, scale);
+        for (int q = 0; q < 4; ++q) c[q] = mx_codes8(v + 8 * q, scale);
         *(u4v*)(codes + ((rt * kt + 4 * b + s) * 64 + lane) * 16) = c;
     }
     __syncthreads();

@@ -37,7 +37,11 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f8u __attribute__((ext_vector_type(8), aligned(4)));
 typedef __bf16 b8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 b4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
 template <class T, int N> struct VecOf;
+template <> struct VecOf<__bf16, 4> { typedef b4u type; };
+template <> struct VecOf<_Float16, 4> { typedef h4u type; };
 template <> struct VecOf<float, 4> { typedef f4u type; };
 template <> struct VecOf<float, 8> { typedef f8u type; };
 template <> struct VecOf<__bf16, 8> { typedef b8u type; };
@@ -77,6 +81,18 @@ __host__ __device__ inline int mx_scale_tiles(int K) { return (int)(((long long)
 inline size_t mx_code_bytes(int rows, int K) { return (size_t)mx_row_tiles(rows) * mx_k_tiles(K) * 1024; }
 inline size_t mx_scale_bytes(int rows, int K) { return (size_t)mx_row_tiles(rows) * mx_scale_tiles(K) * 256; }
 
+// Eight values -> eight codes.
+__device__ __forceinline__ unsigned mx_codes8(const float* v, float scale) {
+    unsigned r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], scale, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], scale, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], scale, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], scale, 3);
+    return r;
+}
+__device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned bits_abs(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
 // A block's scale byte from the bits of max|x| as fp32 (the largest of the
 // values' bit patterns without sign: NaN and infinity are the largest).
 __device__ __forceinline__ unsigned mx_scale_byte(unsigned amax) {
@@ -86,6 +102,20 @@ __device__ __forceinline__ unsigned mx_scale_byte(unsigned amax) {
 // 2^(byte - 127); the hardware's conversions read the exponent of this.
 __device__ __forceinline__ float mx_scale_float(unsigned byte) {
     return __uint_as_float(byte ? byte << 23 : 0x400000u);
+}
+
+// Eight values of a block that four neighbouring lanes hold: the block's scale byte
+// and the lane's codes.
+template <class V>
+__device__ __forceinline__ unsigned mx_codes_of4(const V& v, unsigned& byte) {
+    float f[8];
+    unsigned top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)v[e], top = umax(top, bits_abs(f[e]));
+    top = umax(top, lane_perm<kXor1>(top));
+    top = umax(top, lane_perm<kXor2>(top));
+    byte = mx_scale_byte(top);
+    return mx_codes8(f, mx_scale_float(byte == 255 ? 0 : byte));
 }
 
 // k_mx.hip

@@ -281,8 +281,8 @@ int acfun_dev_quantize_mxfp4(const void* x, int type, int rows, int K, int trans
 /* The values an operand stands for, as x [rows, K]. */
 int acfun_dev_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, int rows, int K, void* x,
                                int type, void* stream);
-/* C[M,N] = A * B^T (+ bias[n], NULL = none; ReLU if act), A an operand of M rows,
- * B of N rows; C of `type`.  K = 0 gives the bias alone. */
+/* C[M,N] = A * B^T (+ bias[n], NULL = none; ReLU if act, NaN staying NaN), A an
+ * operand of M rows, B of N rows; C of `type`.  K = 0 gives the bias alone. */
 int acfun_dev_gemm_mxfp4(int M, int N, int K, const uint8_t* A, const uint8_t* a_scales,
                          const uint8_t* B, const uint8_t* b_scales, void* C, int type,
                          const float* bias, int act, void* stream);

@@ -169,6 +169,16 @@ def test_gemm(gpu, rng, M, N, K, t):
     _check_product(got, layers.mx_decode(*a, K), layers.mx_decode(*b, K), bias, act, t)
 
 
+@pytest.mark.parametrize("t,M,N,K", [("f32", 3600, 4100, 200), ("bf16", 3585, 4097, 1), ("f16", 4096, 4096, 513),
+                                     ("bf16", 20000, 1000, 700)])
+def test_gemm_large(gpu, rng, M, N, K, t):
+    """The largest tiles, whole and cut at both edges."""
+    a, b = _operand(rng, M, K, 3), _operand(rng, N, K, 3)
+    bias = rng.standard_normal(N).astype(np.float32)
+    got = _gemm(gpu, a, b, bias, 0, t, M, N, K)
+    _check_product(got, layers.mx_decode(*a, K), layers.mx_decode(*b, K), bias, 0, t)
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 48, 512), (20, 100, 1000), (300, 600, 640)])
 def test_gemm_bad_blocks(gpu, rng, M, N, K):
     """A NaN block makes its row (or column) of C NaN and nothing else."""
