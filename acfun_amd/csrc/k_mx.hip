@@ -9,7 +9,6 @@
 namespace acfun {
 namespace {
 
-typedef unsigned u4v __attribute__((ext_vector_type(4)));
 
 // Rows along K.  A workgroup: one scale tile, 16 rows x 512 k.  Thread (r, j, p) has
 // the values 8 p .. 8 p + 7 of block j of row r of each of the four 128 k, so 16

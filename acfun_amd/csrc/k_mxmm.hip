@@ -62,35 +62,45 @@ struct MmArgs {
 
 // ---------------------------------------------------------------- few rows
 // 16 TM x 16 TN of C by W waves that split K between them, U 128-k tiles at a time,
-// each from memory to its registers, and add up through LDS: nothing is read
-// twice, and all of a short K is under way at once.  X not void: A is at most 16
-// float rows, and a wave quantizes what it multiplies.
+// and add up through LDS: all of a short K is under way at once.  B comes from
+// memory to registers, and so does A if X is void.  Otherwise A is float rows of X,
+// which the workgroup quantizes into LDS for its tile, while B's first loads are on
+// their way.
+template <class X, int TM, int TN, int W>
+__host__ __device__ inline size_t few_lds(int K) {
+    return (size_t)W * TM * TN * 68 * 16 + (std::is_void_v<X> ? 0 : (size_t)TM * mx_scale_tiles(K) * (4096 + 256));
+}
+
 template <class T, class X, int TM, int TN, int W, int U>
 __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
     constexpr bool ROWS = !std::is_void_v<X>;
-    static_assert(!ROWS || (TM == 1 && U == 4), "a wave's rows are quantized 512 k at a time");
-    __shared__ f4v red[W][TM * TN][64];
-    __shared__ __attribute__((aligned(16))) char quant[ROWS ? W : 1][ROWS ? 4096 + 256 : 1];
+    // partial sums: 16 lanes' quads, and one more, so that the threads of a row read 16
+    // different banks; then the quantized rows: codes, scales
+    extern __shared__ __attribute__((aligned(16))) char smx[];
+    f4v(*const red)[TM * TN][68] = (f4v(*)[TM * TN][68])smx;
+    char* const rc = smx + W * TM * TN * 68 * 16;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned total = (unsigned)p.gm * p.gn, L = xcd_tile(total);
     if (L >= total) return;
-    const int tn = (int)(L / p.gm), tm = (int)(L - (unsigned)tn * p.gm);
-    const int kt = mx_k_tiles(p.K), st = mx_scale_tiles(p.K), units = (kt + U - 1) / U;
-    const long long mt = mx_row_tiles(p.M) - 1, nt = mx_row_tiles(p.N) - 1;
-    const i4v *a[TM], *b[TN];
-    const unsigned *as[TM], *bs[TN];
+    const unsigned tn = p.gm == 1 ? L : L / p.gm, tm = L - tn * p.gm;
+    const unsigned kt = mx_k_tiles(p.K), st = mx_scale_tiles(p.K), units = (kt + U - 1) / U;
+    const unsigned mt = (unsigned)mx_row_tiles(p.M) - 1, nt = (unsigned)mx_row_tiles(p.N) - 1;
+    char* const rs = rc + TM * st * 4096;
+    const uint8_t *a[TM], *as[TM], *b[TN], *bs[TN];             // (uniform)
+    if constexpr (!ROWS)
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const long long t = (long long)tm * TM + i < mt ? (long long)tm * TM + i : mt;
-        a[i] = (const i4v*)p.A + t * kt * 64 + lane;
-        as[i] = (const unsigned*)p.As + t * st * 64 + lane;
-    }
+        for (int i = 0; i < TM; ++i) {
+            const unsigned t = tm * TM + i < mt ? tm * TM + i : mt;
+            a[i] = (const uint8_t*)p.A + ((uint64_t)t * kt << 10);
+            as[i] = p.As + ((uint64_t)t * st << 8);
+        }
 #pragma unroll
     for (int i = 0; i < TN; ++i) {
-        const long long t = (long long)tn * TN + i < nt ? (long long)tn * TN + i : nt;
-        b[i] = (const i4v*)p.B + t * kt * 64 + lane;
-        bs[i] = (const unsigned*)p.Bs + t * st * 64 + lane;
+        const unsigned t = tn * TN + i < nt ? tn * TN + i : nt;
+        b[i] = p.B + ((uint64_t)t * kt << 10);
+        bs[i] = p.Bs + ((uint64_t)t * st << 8);
     }
+    const unsigned o16 = lane * 16u, o4 = lane * 4u;
     f4v acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -100,60 +110,73 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
         i4v a[U][TM], b[U][TN];
         unsigned sa[TM], sb[TN];
     };
-    auto load = [&](Unit& r, int u) {
+    auto load = [&](Unit& r, unsigned u) {
+        const uint64_t g = (uint64_t)(u * U >> 2) << 8;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const long long k = (u * U + i < kt ? u * U + i : kt - 1) * 64ll;
+            const uint64_t k = (uint64_t)(u * U + i < kt ? u * U + i : kt - 1) << 10;
 #pragma unroll
-            for (int j = 0; j < TN; ++j) r.b[i][j] = b[j][k];
+            for (int j = 0; j < TN; ++j) r.b[i][j] = *(const i4v*)(b[j] + k + o16);
             if constexpr (!ROWS)
 #pragma unroll
-                for (int j = 0; j < TM; ++j) r.a[i][j] = a[j][k];
+                for (int j = 0; j < TM; ++j) r.a[i][j] = *(const i4v*)(a[j] + k + o16);
         }
-        const long long g = (u * U >> 2) * 64ll;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) r.sb[j] = bs[j][g];
+        for (int j = 0; j < TN; ++j) r.sb[j] = *(const unsigned*)(bs[j] + g + o4);
         if constexpr (!ROWS)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) r.sa[j] = as[j][g];
+            for (int j = 0; j < TM; ++j) r.sa[j] = *(const unsigned*)(as[j] + g + o4);
     };
-    // 512 k of the float rows through the wave's own LDS: eight values to a lane
-    auto quantize = [&](Unit& r, int u) {
+    // Row by row, 512 k at a time, eight values to a lane: four of these pieces to a wave
+    // at once.  Rows past M are left as they are, for rows of C that are not stored.
+    auto quantize = [&] {
         if constexpr (ROWS) {
-            char* const q = quant[w];
-            const int k = 8 * lane, left = p.K - 512 * u;
-            const int slot = 16 * ((lane >> 2) & 3), s = lane >> 4, part = lane & 3;
-            for (int m0 = 0; m0 < p.M; m0 += 4) {
+            const unsigned rows = (unsigned)p.M - tm * (16 * TM) < 16 * TM ? p.M - tm * (16 * TM) : 16 * TM;
+            const unsigned du = W / rows, dm = W % rows;        // from a wave's piece to its next
+            unsigned u = w / rows, m = w - u * rows;
+            const unsigned slot = 16 * ((lane >> 2) & 3), s = lane >> 4, part = lane & 3;
+            const X* const x = (const X*)p.A + (uint64_t)tm * (16 * TM) * (unsigned)p.K;
+            while (u < st) {
                 typename VecOf<X, 8>::type v[4];
+                unsigned at[4], us[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    us[i] = u, at[i] = m;
+                    if (u < st)
+                        v[i] = load_vec<X, 8>(x + (uint64_t)m * (unsigned)p.K + 512ull * u + 8 * lane,
+                                              p.K - (int)(512 * u) - 8 * lane);
+                    u += du, m += dm;
+                    if (m >= rows) m -= rows, ++u;
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (m0 + i < p.M)
-                        v[i] = load_vec<X, 8>((const X*)p.A + (size_t)(m0 + i) * p.K + 512ll * u + k, left - k);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (m0 + i < p.M) {
+                    if (us[i] < st) {
                         unsigned byte;
                         const unsigned c = mx_codes_of4(v[i], byte);
-                        *(unsigned*)(q + s * 1024 + (slot + m0 + i) * 16 + 4 * part) = c;
-                        if (part == 0) q[4096 + 4 * (slot + m0 + i) + s] = (char)byte;
+                        const unsigned t = (TM == 1 ? 0 : (at[i] >> 4) * st) + us[i], r = slot + (at[i] & 15);
+                        *(unsigned*)(rc + (t * 4 + s) * 1024 + r * 16 + 4 * part) = c;
+                        if (part == 0) rs[t * 256 + 4 * r + s] = (char)byte;
                     }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            // rows past M: whatever is there, for rows of C that are not stored
-#pragma unroll
-            for (int i = 0; i < U; ++i) r.a[i][0] = *(const i4v*)(q + i * 1024 + lane * 16);
-            r.sa[0] = *(const unsigned*)(q + 4096 + 4 * lane);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            __syncthreads();
         }
+    };
+    auto take_rows = [&](Unit& r, unsigned u) {
+        if constexpr (ROWS)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+#pragma unroll
+                for (int i = 0; i < U; ++i) r.a[i][j] = *(const i4v*)(rc + (j * st * 4 + u * U + i) * 1024 + o16);
+                r.sa[j] = *(const unsigned*)(rs + (j * st + (u * U >> 2)) * 256 + o4);
+            }
     };
     Unit r;
     if (w < units) load(r, w);
-    for (int u = w; u < units; u += W) {
+    quantize();
+    for (unsigned u = w; u < units; u += W) {
         Unit c = r;
         if (u + W < units) load(r, u + W);
-        quantize(c, u);
+        take_rows(c, u);
         if constexpr (U < 4) {
             const int sh = 8 * ((u * U) & 3);
 #pragma unroll
@@ -175,17 +198,19 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
 #pragma unroll
     for (int y = 0; y < TM; ++y)
 #pragma unroll
-        for (int x = 0; x < TN; ++x) red[w][y * TN + x][lane] = acc[y][x];
+        for (int x = 0; x < TN; ++x) red[w][y * TN + x][lane + (lane >> 4)] = acc[y][x];
     __syncthreads();
     const float lo = p.act ? 0.f : -__builtin_inff();
-    for (int t = threadIdx.x; t < TM * TN * 64; t += 64 * W) {
-        const int m = t / (4 * TN), q = t - m * 4 * TN;
-        const long long row = (long long)tm * 16 * TM + m, n = (long long)tn * 16 * TN + 4 * q;
-        if (row >= p.M || n >= p.N) continue;
-        const int tile = (m >> 4) * TN + (q >> 2), at = 16 * (q & 3) + (m & 15);
-        f4v v = red[0][tile][at];
+    // four columns of a row to a thread
 #pragma unroll
-        for (int i = 1; i < W; ++i) v += red[i][tile][at];
+    for (int t0 = 0; t0 < TM * TN * 64; t0 += 64 * W) {
+        const int t = t0 + threadIdx.x, m = t / (4 * TN), q = t % (4 * TN);
+        const unsigned row = tm * (16 * TM) + m, n = tn * (16 * TN) + 4 * q;
+        if (t >= TM * TN * 64 || row >= (unsigned)p.M || n >= (unsigned)p.N) continue;
+        const f4v* const from = &red[0][(m >> 4) * TN + (q >> 2)][17 * (q & 3) + (m & 15)];
+        f4v v = from[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) v += from[i * TM * TN * 68];
         const int left = (int)(p.N - n < 4 ? p.N - n : 4);
         if (p.bias) {
             const auto bv = load_vec<float, 4>(p.bias + n, left);
@@ -193,7 +218,7 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
             for (int e = 0; e < 4; ++e) v[e] += bv[e];
         }
         const float o[4] = {at_least(v[0], lo), at_least(v[1], lo), at_least(v[2], lo), at_least(v[3], lo)};
-        store_vec<T, 4>((T*)p.C + row * p.N + n, left, o);
+        store_vec<T, 4>((T*)p.C + (uint64_t)row * (unsigned)p.N + n, left, o);
     }
 }
 
@@ -394,7 +419,8 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void k_mxmm(MmArgs p) {
     typedef typename VecOf<T, CV>::type tvu;
     T* const slab = (T*)smx + wave * SLABS * 32 * RS;
     const long long n0 = (long long)tn * Tl::BN + wn * 32 * FN, m0 = (long long)tm * Tl::BM + wm * 32 * FM;
-    const bool whole = n0 + 32 * FN <= p.N;                 // (uniform)
+    const int cl = lane % LPR * CV;                         // this lane's columns, and how many of them there are
+    const int left = n0 + cl < p.N ? (int)(p.N - n0 - cl < CV ? p.N - n0 - cl : CV) : 0;
     each<FM / SLABS>([&](auto G) {
         constexpr int g = decltype(G)::value * SLABS;
         each<SLABS * FN * 4>([&](auto E) {
@@ -409,18 +435,14 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void k_mxmm(MmArgs p) {
         const long long m = m0 + 32 * g;
         const int rows = p.M - m < 32 * SLABS ? (int)(p.M - m) : 32 * SLABS;
         T* const C = (T*)p.C + m * p.N + n0;
-        if (whole) {
-            const int cl = lane % LPR * CV;
+        if (left == CV)
 #pragma unroll 8
             for (int r = lane / LPR; r < rows; r += RPI)
                 *(tvu*)(C + (size_t)r * p.N + cl) = *(const tv*)(slab + r * RS + cl);
-        } else {
+        else if (left > 0)                                  // the last columns
 #pragma unroll 1
-            for (int t = lane; t < SLABS * 32 * 32 * FN; t += 64) {
-                const int r = t / (32 * FN), c = t % (32 * FN);
-                if (r < rows && n0 + c < p.N) C[(size_t)r * p.N + c] = slab[r * RS + c];
-            }
-        }
+            for (int r = lane / LPR; r < rows; r += RPI)
+                for (int e = 0; e < left; ++e) C[(size_t)r * p.N + cl + e] = slab[r * RS + cl + e];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     });
@@ -428,6 +450,13 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void k_mxmm(MmArgs p) {
 
 template <class T, class X, int TM, int TN, int W, int U>
 bool launch_few(MmArgs a, hipStream_t s) {
+    // set once per process, thread-safely, before any launch below
+    static const bool attr = [] {
+        (void)hipFuncSetAttribute((const void*)k_mxmm_few<T, X, TM, TN, W, U>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        return true;
+    }();
+    (void)attr;
     a.gm = (int)((mx_row_tiles(a.M) + TM - 1) / TM);
     a.gn = (int)((mx_row_tiles(a.N) + TN - 1) / TN);
     const long long grid = ((long long)a.gm * a.gn + 7) / 8 * 8;
@@ -435,7 +464,8 @@ bool launch_few(MmArgs a, hipStream_t s) {
         set_error("acfun_dev_gemm_mxfp4: too large");
         return false;
     }
-    ACFUN_LAUNCH("k_mxmm_few", (k_mxmm_few<T, X, TM, TN, W, U>), dim3((unsigned)grid), dim3(64 * W), 0, s, a);
+    ACFUN_LAUNCH("k_mxmm_few", (k_mxmm_few<T, X, TM, TN, W, U>), dim3((unsigned)grid), dim3(64 * W),
+                 (few_lds<X, TM, TN, W>(a.K)), s, a);
     return check_launch("k_mxmm_few");
 }
 
@@ -481,7 +511,7 @@ bool mx_gemm(int M, int N, int K, const uint8_t* A, const uint8_t* As, const uin
 
 bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_t* Bs, const float* bias,
            int N, void* C, int act, hipStream_t s) {
-    if (M <= 16 && K > 0) {
+    if (K > 0 && M <= 16 && few_lds<float, 1, 1, 8>(K) <= 160 * 1024) {
         const MmArgs a{M, N, K, x, nullptr, B, Bs, C, bias, act, 0, 0};
         return with_type(type, [&](auto t) {
             using T = decltype(t);

@@ -105,17 +105,52 @@ __device__ __forceinline__ float mx_scale_float(unsigned byte) {
 }
 
 // Eight values of a block that four neighbouring lanes hold: the block's scale byte
-// and the lane's codes.
-template <class V>
-__device__ __forceinline__ unsigned mx_codes_of4(const V& v, unsigned& byte) {
+// and the lane's codes.  The 16-bit types find their maximum and are converted as
+// pairs, with half the instructions.
+__device__ __forceinline__ unsigned max_of4(unsigned top) {
+    top = umax(top, lane_perm<kXor1>(top));
+    return umax(top, lane_perm<kXor2>(top));
+}
+__device__ __forceinline__ unsigned mx_codes_of4(const f8u& v, unsigned& byte) {
     float f[8];
     unsigned top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (float)v[e], top = umax(top, bits_abs(f[e]));
-    top = umax(top, lane_perm<kXor1>(top));
-    top = umax(top, lane_perm<kXor2>(top));
-    byte = mx_scale_byte(top);
+    for (int e = 0; e < 8; ++e) f[e] = v[e], top = umax(top, bits_abs(f[e]));
+    byte = mx_scale_byte(max_of4(top));
     return mx_codes8(f, mx_scale_float(byte == 255 ? 0 : byte));
+}
+typedef unsigned u4v __attribute__((ext_vector_type(4)));
+// (by value: a bit_cast of a vector's element itself would read element 0)
+template <class P>
+__device__ __forceinline__ P as_pair(unsigned u) { return __builtin_bit_cast(P, u); }
+__device__ __forceinline__ unsigned max16_of4(const u4v& v) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    auto abs2 = [](unsigned u) { return as_pair<us2>(u & 0x7fff7fffu); };
+    const us2 m = __builtin_elementwise_max(__builtin_elementwise_max(abs2(v[0]), abs2(v[1])),
+                                            __builtin_elementwise_max(abs2(v[2]), abs2(v[3])));
+    return max_of4(umax(m[0], m[1]));
+}
+__device__ __forceinline__ unsigned mx_codes_of4(const b8u& v, unsigned& byte) {
+    typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+    const u4v u = __builtin_bit_cast(u4v, v);
+    byte = mx_scale_byte(max16_of4(u) << 16);
+    const float scale = mx_scale_float(byte == 255 ? 0 : byte);
+    unsigned r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_pair<b2v>(u[0]), scale, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_pair<b2v>(u[1]), scale, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_pair<b2v>(u[2]), scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_pair<b2v>(u[3]), scale, 3);
+}
+__device__ __forceinline__ unsigned mx_codes_of4(const h8u& v, unsigned& byte) {
+    typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+    const u4v u = __builtin_bit_cast(u4v, v);
+    byte = mx_scale_byte(__float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)max16_of4(u))));
+    const float scale = mx_scale_float(byte == 255 ? 0 : byte);
+    unsigned r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_pair<h2v>(u[0]), scale, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_pair<h2v>(u[1]), scale, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_pair<h2v>(u[2]), scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_pair<h2v>(u[3]), scale, 3);
 }
 
 // k_mx.hip
