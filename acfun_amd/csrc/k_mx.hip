@@ -61,8 +61,8 @@ __global__ __launch_bounds__(256) void k_mx_quant_t(const T* __restrict__ x, int
     for (int e = 0; e < 32; ++e) v[e] = row < (unsigned)rows && k0 + e < left ? (float)xk[(size_t)e * rows] : 0.f;
 #pragma unroll
     for (int e = 0; e < 32; ++e) top = umax(top, bits_abs(v[e]));
-    const unsigned byte = mx_scale_byte(top);
-    const float scale = mx_scale_float(byte == 255 ? 0 : byte);
+    float scale;
+    const unsigned byte = mx_scale(top >> 23, scale);
     bytes[s][l] = byte;
     const size_t rt = row >> 4, lane = 16 * j + (row & 15);
     const bool tile = row < (((unsigned)rows + 15) & ~15u);

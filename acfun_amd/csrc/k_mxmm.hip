@@ -74,6 +74,7 @@ __host__ __device__ inline size_t few_lds(int K) {
 template <class T, class X, int TM, int TN, int W, int U>
 __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
     constexpr bool ROWS = !std::is_void_v<X>;
+    using E = std::conditional_t<ROWS, X, float>;
     // partial sums: 16 lanes' quads, and one more, so that the threads of a row read 16
     // different banks; then the quantized rows: codes, scales
     extern __shared__ __attribute__((aligned(16))) char smx[];
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
         b[i] = p.B + ((uint64_t)t * kt << 10);
         bs[i] = p.Bs + ((uint64_t)t * st << 8);
     }
-    const unsigned o16 = lane * 16u, o4 = lane * 4u;
+    const unsigned o16 = lane * 16u, o4 = lane * 4u, oq = (lane ^ (lane >> 4)) * 16u;
     f4v acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -127,38 +128,43 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
 #pragma unroll
             for (int j = 0; j < TM; ++j) r.sa[j] = *(const unsigned*)(as[j] + g + o4);
     };
-    // Row by row, 512 k at a time, eight values to a lane: four of these pieces to a wave
-    // at once.  Rows past M are left as they are, for rows of C that are not stored.
-    auto quantize = [&] {
-        if constexpr (ROWS) {
-            const unsigned rows = (unsigned)p.M - tm * (16 * TM) < 16 * TM ? p.M - tm * (16 * TM) : 16 * TM;
-            const unsigned du = W / rows, dm = W % rows;        // from a wave's piece to its next
-            unsigned u = w / rows, m = w - u * rows;
-            const unsigned slot = 16 * ((lane >> 2) & 3), s = lane >> 4, part = lane & 3;
-            const X* const x = (const X*)p.A + (uint64_t)tm * (16 * TM) * (unsigned)p.K;
-            while (u < st) {
-                typename VecOf<X, 8>::type v[4];
-                unsigned at[4], us[4];
+    // Pieces of a row and 512 k, eight values to a lane; Q pieces to a wave at once, for
+    // the latency of their loads (the kernel's first call runs through code that is
+    // not in its cache: rows that end inside a lane's eight values have their own,
+    // shorter, loop).  Rows past M are left as they are, for rows of C that are not
+    // stored.  Codes lie as in an operand but for the place of row r in block j of the
+    // s-th 128 k, which is r ^ (4 s + j): a piece's blocks are written to different banks.
+    auto quantize = [&](auto QC, auto whole) {
+        constexpr int Q = decltype(QC)::value;
+        const unsigned rows = (unsigned)p.M - tm * (16 * TM) < 16 * TM ? p.M - tm * (16 * TM) : 16 * TM;
+        const unsigned du = W / rows, dm = W % rows;            // from a wave's piece to its next
+        unsigned u = w / rows, m = w - u * rows;
+        const unsigned j = (lane >> 2) & 3, s = lane >> 4, part = lane & 3;
+        const E* const x = (const E*)p.A + (uint64_t)tm * (16 * TM) * (unsigned)p.K;
+        while (u < st) {
+            typename VecOf<E, 8>::type v[Q] = {};
+            unsigned to[Q], us[Q];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    us[i] = u, at[i] = m;
-                    if (u < st)
-                        v[i] = load_vec<X, 8>(x + (uint64_t)m * (unsigned)p.K + 512ull * u + 8 * lane,
-                                              p.K - (int)(512 * u) - 8 * lane);
-                    u += du, m += dm;
-                    if (m >= rows) m -= rows, ++u;
+            for (int i = 0; i < Q; ++i) {
+                us[i] = u;
+                to[i] = TM == 1 ? m : (m >> 4) * st * 256 + (m & 15);
+                if (u < st) {
+                    const E* const from = x + (uint64_t)m * (unsigned)p.K + 512ull * u;
+                    const int left = p.K - (int)(512 * u) - 8 * lane;
+                    if constexpr (!decltype(whole)::value) v[i] = load_vec<E, 8>(from + 8u * lane, left);
+                    else if (left > 0) v[i] = *(const typename VecOf<E, 8>::type*)(from + 8u * lane);
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (us[i] < st) {
-                        unsigned byte;
-                        const unsigned c = mx_codes_of4(v[i], byte);
-                        const unsigned t = (TM == 1 ? 0 : (at[i] >> 4) * st) + us[i], r = slot + (at[i] & 15);
-                        *(unsigned*)(rc + (t * 4 + s) * 1024 + r * 16 + 4 * part) = c;
-                        if (part == 0) rs[t * 256 + 4 * r + s] = (char)byte;
-                    }
+                u += du, m += dm;
+                if (m >= rows) m -= rows, ++u;
             }
-            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < Q; ++i)
+                if (us[i] < st) {
+                    unsigned byte;
+                    const unsigned c = mx_codes_of4(v[i], byte), t = (to[i] & ~255u) + us[i] * 256, r = to[i] & 15;
+                    *(unsigned*)(rc + t * 16 + s * 1024 + j * 256 + (r ^ (4 * s + j)) * 16 + 4 * part) = c;
+                    if (part == 0) rs[t + 64 * j + 4 * r + s] = (char)byte;
+                }
         }
     };
     auto take_rows = [&](Unit& r, unsigned u) {
@@ -166,13 +172,18 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
 #pragma unroll
             for (int j = 0; j < TM; ++j) {
 #pragma unroll
-                for (int i = 0; i < U; ++i) r.a[i][j] = *(const i4v*)(rc + (j * st * 4 + u * U + i) * 1024 + o16);
+                for (int i = 0; i < U; ++i)
+                    r.a[i][j] = *(const i4v*)(rc + (j * st * 4 + u * U + i) * 1024 + (oq ^ ((u * U + i) & 3) * 64));
                 r.sa[j] = *(const unsigned*)(rs + (j * st + (u * U >> 2)) * 256 + o4);
             }
     };
     Unit r;
     if (w < units) load(r, w);
-    quantize();
+    if constexpr (ROWS) {
+        if (p.K % 8 == 0) quantize(std::integral_constant<int, 4>{}, std::true_type{});
+        else quantize(std::integral_constant<int, 2>{}, std::false_type{});
+        __syncthreads();
+    }
     for (unsigned u = w; u < units; u += W) {
         Unit c = r;
         if (u + W < units) load(r, u + W);
@@ -490,6 +501,52 @@ bool launch_many(MmArgs a, hipStream_t s) {
     return check_launch("k_mxmm");
 }
 
+// Times in us that choose a kernel and its tile, fitted to those of every tile over
+// 518 sizes (M of 16 to 8192, N of 64 to 8192, K of 128 to 8192; bf16, replayed from a
+// graph): a call takes `lat` while the CUs have less than a tile each, and `base` and
+// `each` times the tiles of a CU from there.  The tile chosen is 1.4 % slower than the
+// best of each size in the mean.  Measured, us: 128 x 8192 x 4096 9.7 with tiles of 32,
+// 6.8 with 64, 11.3 with 128; 512 x 8192 x 1024 15 with 64, 7.1 with 128; 2048 x 8192 x
+// 4096 45 with 128, 39 with 256.
+double tile_time(double lat, double base, double each, double tiles_per_cu) {
+    const double t = base + each * tiles_per_cu;
+    return t > lat ? t : lat;
+}
+
+enum MmKind { FEW16, FEW32, FEW64, MANY128, MANY256, KINDS };
+
+// The fastest kernel for a product, and its time.
+MmKind mm_choose(int M, int N, int K, double& us) {
+    const double cus = num_cus(), k = K;
+    auto per_cu = [&](int b) {
+        return (double)(((long long)M + b - 1) / b) * (double)(((long long)N + b - 1) / b) / cus;
+    };
+    auto more = [](double a, double b) { return a > b ? a : b; };
+    const double t[KINDS] = {
+        tile_time(2.78 + 0.75e-4 * k, 2.1 + 1.2e-4 * k, 0.42 + 1.6e-4 * k, per_cu(16)),
+        tile_time(2.8 + 3.0e-4 * k, 2.65 + 3.2e-4 * k, more(0.28 + 2.75e-4 * k, 3.8e-4 * k), per_cu(32)),
+        tile_time(3.85 + 8.0e-4 * k, 2.15 + 2.9e-4 * k, 2.4 + 8.5e-4 * k, per_cu(64)),
+        tile_time(3.9 + 17.2e-4 * k, 3.6 + 3.3e-4 * k, more(1.9 + 17.8e-4 * k, 20.7e-4 * k), per_cu(128)),
+        tile_time(7.05 + 45.2e-4 * k, 6.0, more(7.0 + 61.7e-4 * k, 72.7e-4 * k), per_cu(256)),
+    };
+    // 32-bit offsets into a tile's operands
+    const int kinds = K > 0 && K <= (1 << 22) ? KINDS : MANY128;
+    int best = 0;
+    for (int i = 1; i < kinds; ++i)
+        if (t[i] < t[best]) best = i;
+    us = t[best];
+    return (MmKind)best;
+}
+
+// The same for a layer whose workgroups each quantize their 16 rows, with tiles of 16,
+// 32 or 64 columns (tn tiles of 16): `pieces` of a row and 512 k fall to each wave.
+double rows_time(int M, int N, int K, int tn) {
+    const double k = K, pieces = (double)(((M < 16 ? M : 16) * (long long)mx_scale_tiles(K) + 7) / 8);
+    const double per_cu = (double)mx_row_tiles(M) * (double)((mx_row_tiles(N) + tn - 1) / tn) / num_cus();
+    return tile_time(2.96 + 0.034 * tn + (0.91e-4 * tn - 0.51e-4) * k + 0.265 * pieces, 2.3 + 0.2 * pieces,
+                     0.42 + 0.124 * tn + (1.44e-4 + 0.91e-4 * tn) * k + 0.1 * pieces, per_cu);
+}
+
 }  // namespace
 
 bool mx_gemm(int M, int N, int K, const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs,
@@ -497,26 +554,39 @@ bool mx_gemm(int M, int N, int K, const uint8_t* A, const uint8_t* As, const uin
     const MmArgs a{M, N, K, A, As, B, Bs, C, bias, act, 0, 0};
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        const long long cus = num_cus();
-        auto tiles = [&](long long m, long long n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
-        if (K > 0 && K <= (1 << 22)) {                      // 32-bit offsets in a tile's operands
-            if (tiles(256, 256) * 8 >= cus * 7) return launch_many<T, 4, 4>(a, s);
-            if (tiles(128, 128) * 8 >= cus * 7) return launch_many<T, 2, 2>(a, s);
+        double us;
+        switch (mm_choose(M, N, K, us)) {
+            case FEW16: return launch_few<T, void, 1, 1, 8, 4>(a, s);
+            case FEW32: return launch_few<T, void, 2, 2, 4, 2>(a, s);
+            case FEW64: return launch_few<T, void, 4, 4, 8, 1>(a, s);
+            case MANY128: return launch_many<T, 2, 2>(a, s);
+            default: return launch_many<T, 4, 4>(a, s);
         }
-        if (tiles(64, 64) * 8 >= cus * 7) return launch_few<T, void, 4, 4, 8, 1>(a, s);
-        if (tiles(32, 32) * 8 >= cus * 7) return launch_few<T, void, 2, 2, 8, 2>(a, s);
-        return launch_few<T, void, 1, 1, 8, 4>(a, s);
     });
 }
 
 bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_t* Bs, const float* bias,
            int N, void* C, int act, hipStream_t s) {
-    if (K > 0 && M <= 16 && few_lds<float, 1, 1, 8>(K) <= 160 * 1024) {
-        const MmArgs a{M, N, K, x, nullptr, B, Bs, C, bias, act, 0, 0};
-        return with_type(type, [&](auto t) {
-            using T = decltype(t);
-            return launch_few<T, T, 1, 1, 8, 4>(a, s);
-        });
+    if (K > 0 && few_lds<float, 1, 4, 8>(K) <= 160 * 1024) {
+        // One launch, in which every workgroup quantizes its 16 rows, or two, of which the
+        // first takes 2.5 us and its traffic at 4 TB/s?  Measured, us: 16 x 2048 x 2048 5.0 and
+        // 5.1, 16 x 2048 x 4096 7.2 and 5.4; 333 x 512 x 1024 4.5 and 6.9, 333 x 2048 x 2048
+        // 11.4 and 8.7.
+        double two, one = rows_time(M, N, K, 1);
+        (void)mm_choose(M, N, K, two);
+        two += 2.5 + (double)M * K * (type_size(type) + 0.53) * 0.25e-6;
+        int tn = 1;
+        for (int n = 2; n <= 4; n *= 2)
+            if (rows_time(M, N, K, n) < one) one = rows_time(M, N, K, tn = n);
+        if (one < two) {
+            const MmArgs a{M, N, K, x, nullptr, B, Bs, C, bias, act, 0, 0};
+            return with_type(type, [&](auto t) {
+                using T = decltype(t);
+                if (tn == 1) return launch_few<T, T, 1, 1, 8, 4>(a, s);
+                if (tn == 2) return launch_few<T, T, 1, 2, 8, 4>(a, s);
+                return launch_few<T, T, 1, 4, 8, 2>(a, s);
+            });
+        }
     }
     Scratch codes(mx_code_bytes(M, K), s), scales(mx_scale_bytes(M, K), s);
     if (K > 0 && (!codes.p || !scales.p)) return false;

@@ -93,13 +93,15 @@ __device__ __forceinline__ unsigned mx_codes8(const float* v, float scale) {
 __device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
 __device__ __forceinline__ unsigned bits_abs(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// A block's scale byte from the bits of max|x| as fp32 (the largest of the
-// values' bit patterns without sign: NaN and infinity are the largest).
-__device__ __forceinline__ unsigned mx_scale_byte(unsigned amax) {
-    const unsigned e = amax >> 23;
-    return e == 255 ? 255u : (e > 2 ? e - 2 : 0u);
+// A block's scale byte, and the scale for the hardware's conversions (which read its
+// exponent), from the exponent field of max|x| as fp32.  255 (a NaN or an infinity is
+// the largest of the values' bit patterns without sign) makes any codes do.
+__device__ __forceinline__ unsigned mx_scale(unsigned e, float& scale) {
+    const unsigned b = e > 2 ? e - 2 : 0;
+    scale = __uint_as_float(b << 23 | 0x400000u);
+    return e == 255 ? 255u : b;
 }
-// 2^(byte - 127); the hardware's conversions read the exponent of this.
+// 2^(byte - 127)
 __device__ __forceinline__ float mx_scale_float(unsigned byte) {
     return __uint_as_float(byte ? byte << 23 : 0x400000u);
 }
@@ -116,8 +118,9 @@ __device__ __forceinline__ unsigned mx_codes_of4(const f8u& v, unsigned& byte) {
     unsigned top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = v[e], top = umax(top, bits_abs(f[e]));
-    byte = mx_scale_byte(max_of4(top));
-    return mx_codes8(f, mx_scale_float(byte == 255 ? 0 : byte));
+    float scale;
+    byte = mx_scale(max_of4(top) >> 23, scale);
+    return mx_codes8(f, scale);
 }
 typedef unsigned u4v __attribute__((ext_vector_type(4)));
 // (by value: a bit_cast of a vector's element itself would read element 0)
@@ -133,8 +136,8 @@ __device__ __forceinline__ unsigned max16_of4(const u4v& v) {
 __device__ __forceinline__ unsigned mx_codes_of4(const b8u& v, unsigned& byte) {
     typedef __bf16 b2v __attribute__((ext_vector_type(2)));
     const u4v u = __builtin_bit_cast(u4v, v);
-    byte = mx_scale_byte(max16_of4(u) << 16);
-    const float scale = mx_scale_float(byte == 255 ? 0 : byte);
+    float scale;
+    byte = mx_scale(max16_of4(u) >> 7, scale);
     unsigned r = 0;
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_pair<b2v>(u[0]), scale, 0);
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_pair<b2v>(u[1]), scale, 1);
@@ -144,8 +147,9 @@ __device__ __forceinline__ unsigned mx_codes_of4(const b8u& v, unsigned& byte) {
 __device__ __forceinline__ unsigned mx_codes_of4(const h8u& v, unsigned& byte) {
     typedef _Float16 h2v __attribute__((ext_vector_type(2)));
     const u4v u = __builtin_bit_cast(u4v, v);
-    byte = mx_scale_byte(__float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)max16_of4(u))));
-    const float scale = mx_scale_float(byte == 255 ? 0 : byte);
+    const _Float16 top = __builtin_bit_cast(_Float16, (unsigned short)max16_of4(u));
+    float scale;
+    byte = mx_scale(__float_as_uint((float)top) >> 23, scale);
     unsigned r = 0;
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_pair<h2v>(u[0]), scale, 0);
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_pair<h2v>(u[1]), scale, 1);
