@@ -13,6 +13,8 @@
 // TB/s; a copy reaches 5.55), the norm of 4096 x 4096 fp16 13.9 us; one token 4.7
 // and 4.9 us, of which the launch is most.  With a value per thread and step
 // and parameters read for every row: 478, 26.1, 5.6 and 21.2.
+#include <type_traits>
+
 #include "mx.hpp"
 
 namespace acfun {
@@ -52,10 +54,14 @@ struct RowSum {
 
 // TPR threads to a row (64: a wave, four rows to a workgroup), CH chunks of 16
 // bytes to a thread.  The row stays in registers, so every value is read once;
-// a workgroup takes rows in turn.  With one or two chunks it keeps the weights and
-// the gate of its columns and has the next row's loads under way (128 registers
-// hold that, for four waves per SIMD); biases are read where they are added.
-template <class T, int TPR, int CH, bool RES, bool LAYER>
+// a workgroup takes rows in turn, `step` apart.  With one or two chunks it keeps the
+// weights and the gate of its columns and has the next row's loads under way (128
+// registers hold that, for four waves per SIMD); biases are read where they are
+// added.  WHOLE: rows are whole chunks, so a thread's chunk is all there or not at
+// all, with half the code: one row's time is for a good part the fetching of it.
+// (gridDim is not asked for: the hidden arguments that it comes with, and any more
+// than 128 bytes of them, cost a launch 0.7 us on the host.)
+template <class T, int TPR, int CH, bool RES, bool WHOLE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs a) {
     constexpr int VN = 16 / (int)sizeof(T), NW = TPR / 64, RPB = TPR == 64 ? 4 : 1;
     constexpr bool KEEP = CH <= 2;
@@ -65,16 +71,23 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
     RowSum<NW> sum{red};
     const int t = threadIdx.x & (TPR - 1), cols = a.cols;
     int row = (int)(blockIdx.x * RPB) + (RPB > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
-    const int step = (int)(gridDim.x * RPB);
     if (row >= a.rows) return;
-    const float* const par[4] = {a.post_w, a.post_b, a.pre_w, a.pre_b};
     auto col = [&](int i) { return (i * TPR + t) * VN; };
-    auto load_par = [&](int q, int i) {
-        const float fill = q & 1 ? 0.f : 1.f;
-        P v;
-#pragma unroll
-        for (int e = 0; e < VN; ++e) v[e] = fill;
-        return par[q] ? load_vec<float, VN>(par[q] + col(i), cols - col(i), fill) : v;
+    auto get = [&](const T* p, int i) {
+        V v = {};
+        if constexpr (!WHOLE) v = load_vec<T, VN>(p + col(i), cols - col(i));
+        else if (col(i) < cols) v = *(const V*)(p + col(i));
+        return v;
+    };
+    auto get_par = [&](const float* p, int i) {
+        P v = {};
+        if constexpr (!WHOLE) v = load_vec<float, VN>(p + col(i), cols - col(i));
+        else if (col(i) < cols) v = *(const P*)(p + col(i));
+        return v;
+    };
+    auto put = [&](T* p, int i, const float (&v)[VN]) {
+        if constexpr (!WHOLE) store_vec<T, VN>(p + col(i), cols - col(i), v);
+        else if (col(i) < cols) store_vec<T, VN>(p + col(i), VN, v);
     };
     V yv[CH], xv[CH], gv[KEEP ? CH : 1];           // a row of x beside y: KEEP only
     int group = -1;
@@ -82,13 +95,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
         const size_t at = (size_t)r * cols;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            if constexpr (RES) yv[i] = load_vec<T, VN>((const T*)a.y + at + col(i), cols - col(i));
-            if constexpr (!RES || KEEP) xv[i] = load_vec<T, VN>((const T*)a.x + at + col(i), cols - col(i));
+            if constexpr (RES) yv[i] = get((const T*)a.y + at, i);
+            if constexpr (!RES || KEEP) xv[i] = get((const T*)a.x + at, i);
         }
     };
-    auto gate_vec = [&](int i) {
-        return load_vec<T, VN>((const T*)a.gate + (size_t)group * cols + col(i), cols - col(i));
-    };
+    auto gate_vec = [&](int i) { return get((const T*)a.gate + (size_t)group * cols, i); };
     auto load_gate = [&](int r) {
         if (!RES || !a.gate || r / a.gate_group == group) return;
         group = r / a.gate_group;
@@ -102,49 +113,63 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
     P kept[2][KEEP ? CH : 1];
     if constexpr (KEEP) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            if constexpr (RES) kept[0][i] = load_par(0, i);
-            kept[1][i] = load_par(2, i);
-        }
+        for (int q = RES ? 0 : 1; q < 2; ++q)
+            if (const float* const w = q ? a.pre_w : a.post_w) {
+#pragma unroll
+                for (int i = 0; i < CH; ++i) kept[q][i] = get_par(w, i);
+            }
     }
     // (n * weight + bias) of chunk i, in place
-    auto scale = [&](int q, int i, float (&n)[VN]) {
-        P w;
-        if constexpr (KEEP) w = kept[q >> 1][i];
-        else w = load_par(q, i);
+    auto scale = [&](auto Q, int i, float (&n)[VN]) {
+        constexpr int q = decltype(Q)::value;
+        const float *const pw = q ? a.pre_w : a.post_w, *const pb = q ? a.pre_b : a.post_b;
+        if (pw) {
+            P w;
+            if constexpr (KEEP) w = kept[q][i];
+            else w = get_par(pw, i);
 #pragma unroll
-        for (int e = 0; e < VN; ++e) n[e] *= w[e];
-        if (!par[q + 1]) return;
-        const P b = load_par(q + 1, i);
+            for (int e = 0; e < VN; ++e) n[e] *= w[e];
+        }
+        if (pb) {
+            const P b = get_par(pb, i);
 #pragma unroll
-        for (int e = 0; e < VN; ++e) n[e] += b[e];
+            for (int e = 0; e < VN; ++e) n[e] += b[e];
+        }
     };
     const float inv = 1.f / (float)cols;
     float v[CH][VN];
+    auto in = [&](int i, int e) { return WHOLE ? col(i) < cols : col(i) + e < cols; };
     auto stats = [&](float& mean, float& rs) {
         mean = 0.f;
-        if constexpr (LAYER) {
+        float q = 0.f;
+        if (a.layer) {
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < CH; ++i)
 #pragma unroll
                 for (int e = 0; e < VN; ++e) s += v[i][e];         // 0 past the row's end
             mean = sum(s) * inv;
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+#pragma unroll
+                for (int e = 0; e < VN; ++e) {
+                    const float d = in(i, e) ? v[i][e] - mean : 0.f;
+                    q = fmaf(d, d, q);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+#pragma unroll
+                for (int e = 0; e < VN; ++e) q = fmaf(v[i][e], v[i][e], q);
         }
-        float q = 0.f;
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-#pragma unroll
-            for (int e = 0; e < VN; ++e) {
-                const float d = !LAYER ? v[i][e] : col(i) + e < cols ? v[i][e] - mean : 0.f;
-                q = fmaf(d, d, q);
-            }
         rs = 1.f / sqrtf(sum(q) * inv + a.eps);
     };
+    using Post = std::integral_constant<int, 0>;
+    using Pre = std::integral_constant<int, 1>;
     for (;;) {
         const size_t at = (size_t)row * cols;
-        const bool more = step < a.rows - row;
-        const int next = more ? row + step : row;
+        const bool more = a.step < a.rows - row;
+        const int next = more ? row + a.step : row;
         float mean, rs;
         if constexpr (RES) {
             V x[CH];
@@ -159,10 +184,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 float n[VN];
-                if constexpr (!KEEP) x[i] = load_vec<T, VN>((const T*)a.x + at + col(i), cols - col(i));
+                if constexpr (!KEEP) x[i] = get((const T*)a.x + at, i);
 #pragma unroll
                 for (int e = 0; e < VN; ++e) n[e] = (v[i][e] - mean) * rs;
-                scale(0, i, n);
+                scale(Post{}, i, n);
                 if (a.gate) {
                     V g;
                     if constexpr (KEEP) g = gv[i];
@@ -171,9 +196,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
                     for (int e = 0; e < VN; ++e) n[e] *= (float)g[e];
                 }
 #pragma unroll
-                for (int e = 0; e < VN; ++e)
-                    v[i][e] = col(i) + e < cols ? a.res_scale * (float)x[i][e] + n[e] : 0.f;
-                store_vec<T, VN>((T*)a.x_out + at + col(i), cols - col(i), v[i]);
+                for (int e = 0; e < VN; ++e) v[i][e] = in(i, e) ? a.res_scale * (float)x[i][e] + n[e] : 0.f;
+                put((T*)a.x_out + at, i, v[i]);
             }
         } else {
 #pragma unroll
@@ -189,8 +213,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
                 float n[VN];
 #pragma unroll
                 for (int e = 0; e < VN; ++e) n[e] = (v[i][e] - mean) * rs;
-                scale(2, i, n);
-                store_vec<T, VN>((T*)a.h + at + col(i), cols - col(i), n);
+                scale(Pre{}, i, n);
+                put((T*)a.h + at, i, n);
             }
         }
         if (!more) break;
@@ -201,15 +225,17 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
 }
 
 template <class T, int TPR, int CH>
-bool launch(const NormArgs& a, hipStream_t s) {
+bool launch(NormArgs a, hipStream_t s) {
     constexpr int RPB = TPR == 64 ? 4 : 1, THREADS = TPR < 256 ? 256 : TPR;
     // at most four waves per SIMD, and as many rows to each workgroup
     const long long groups = ((long long)a.rows + RPB - 1) / RPB, most = num_cus() * (1024 / THREADS);
     const long long each = (groups + most - 1) / most;
     const dim3 grid((unsigned)((groups + each - 1) / each)), block(THREADS);
-    if (a.y && a.layer) ACFUN_LAUNCH("k_norm_row", (k_norm_row<T, TPR, CH, true, true>), grid, block, 0, s, a);
+    a.step = (int)(grid.x * RPB);
+    const bool whole = a.cols % (16 / (int)sizeof(T)) == 0;
+    if (a.y && whole) ACFUN_LAUNCH("k_norm_row", (k_norm_row<T, TPR, CH, true, true>), grid, block, 0, s, a);
     else if (a.y) ACFUN_LAUNCH("k_norm_row", (k_norm_row<T, TPR, CH, true, false>), grid, block, 0, s, a);
-    else if (a.layer) ACFUN_LAUNCH("k_norm_row", (k_norm_row<T, TPR, CH, false, true>), grid, block, 0, s, a);
+    else if (whole) ACFUN_LAUNCH("k_norm_row", (k_norm_row<T, TPR, CH, false, true>), grid, block, 0, s, a);
     else ACFUN_LAUNCH("k_norm_row", (k_norm_row<T, TPR, CH, false, false>), grid, block, 0, s, a);
     return check_launch("k_norm_row");
 }

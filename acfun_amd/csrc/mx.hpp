@@ -180,6 +180,7 @@ struct NormArgs {
     const float *pre_w, *pre_b;     // norm of the sum
     float eps;
     void *x_out, *h;                // h null: no norm of the sum
+    int step = 0;                   // rows from one to the next of a workgroup
 };
 bool norm_rows(const NormArgs& a, int type, hipStream_t s);
 constexpr int kNormMaxCols = 32768;
