@@ -128,44 +128,49 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
 #pragma unroll
             for (int j = 0; j < TM; ++j) r.sa[j] = *(const unsigned*)(as[j] + g + o4);
     };
-    // Pieces of a row and 512 k, eight values to a lane; Q pieces to a wave at once, for
-    // the latency of their loads (the kernel's first call runs through code that is
-    // not in its cache: rows that end inside a lane's eight values have their own,
-    // shorter, loop).  Rows past M are left as they are, for rows of C that are not
-    // stored.  Codes lie as in an operand but for the place of row r in block j of the
-    // s-th 128 k, which is r ^ (4 s + j): a piece's blocks are written to different banks.
-    auto quantize = [&](auto QC, auto whole) {
-        constexpr int Q = decltype(QC)::value;
+    // Pieces of a row and 512 k, eight values to a lane; four to a wave at once, for the
+    // latency of their loads, then one by one.  ENDS: 0 where K is whole pieces, 1 where
+    // it ends between lanes, 2 inside a lane's eight values (a kernel fetches its code
+    // as it goes, so each has its own).  Rows past M are left as they are, for rows of C
+    // that are not stored.  Codes lie as in an operand but for the place of row r in block
+    // j of the s-th 128 k, which is r ^ (4 s + j): a piece's blocks are written to
+    // different banks.
+    auto quantize = [&](auto ENDS) {
+        constexpr int ends = decltype(ENDS)::value;
         const unsigned rows = (unsigned)p.M - tm * (16 * TM) < 16 * TM ? p.M - tm * (16 * TM) : 16 * TM;
         const unsigned du = W / rows, dm = W % rows;            // from a wave's piece to its next
         unsigned u = w / rows, m = w - u * rows;
         const unsigned j = (lane >> 2) & 3, s = lane >> 4, part = lane & 3;
         const E* const x = (const E*)p.A + (uint64_t)tm * (16 * TM) * (unsigned)p.K;
-        while (u < st) {
+        auto some = [&](auto QC) {
+            constexpr int Q = decltype(QC)::value;
             typename VecOf<E, 8>::type v[Q] = {};
-            unsigned to[Q], us[Q];
+            unsigned to[Q], row[Q];
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
-                us[i] = u;
-                to[i] = TM == 1 ? m : (m >> 4) * st * 256 + (m & 15);
-                if (u < st) {
-                    const E* const from = x + (uint64_t)m * (unsigned)p.K + 512ull * u;
-                    const int left = p.K - (int)(512 * u) - 8 * lane;
-                    if constexpr (!decltype(whole)::value) v[i] = load_vec<E, 8>(from + 8u * lane, left);
-                    else if (left > 0) v[i] = *(const typename VecOf<E, 8>::type*)(from + 8u * lane);
-                }
+                to[i] = (TM == 1 ? u : (m >> 4) * st + u) * 256;
+                row[i] = m & 15;
+                const E* const from = x + (uint64_t)m * (unsigned)p.K + 512ull * u;
+                const int left = p.K - (int)(512 * u) - 8 * lane;
+                if constexpr (ends == 2) v[i] = load_vec<E, 8>(from + 8u * lane, left);
+                else if (ends == 0 || left > 0) v[i] = *(const typename VecOf<E, 8>::type*)(from + 8u * lane);
                 u += du, m += dm;
                 if (m >= rows) m -= rows, ++u;
             }
 #pragma unroll
-            for (int i = 0; i < Q; ++i)
-                if (us[i] < st) {
-                    unsigned byte;
-                    const unsigned c = mx_codes_of4(v[i], byte), t = (to[i] & ~255u) + us[i] * 256, r = to[i] & 15;
-                    *(unsigned*)(rc + t * 16 + s * 1024 + j * 256 + (r ^ (4 * s + j)) * 16 + 4 * part) = c;
-                    if (part == 0) rs[t + 64 * j + 4 * r + s] = (char)byte;
-                }
-        }
+            for (int i = 0; i < Q; ++i) {
+                unsigned byte;
+                const unsigned c = mx_codes_of4(v[i], byte);
+                *(unsigned*)(rc + to[i] * 16 + s * 1024 + j * 256 + (row[i] ^ (4 * s + j)) * 16 + 4 * part) = c;
+                // (all four lanes of a block have its scale byte)
+                rs[to[i] + 64 * j + 4 * row[i] + s] = (char)byte;
+            }
+        };
+        const unsigned mine = (rows * st + W - 1 - w) / W;
+        unsigned n = 0;
+        for (; n + 4 <= mine; n += 4) some(std::integral_constant<int, 4>{});
+#pragma unroll 1
+        for (; n < mine; ++n) some(std::integral_constant<int, 1>{});
     };
     auto take_rows = [&](Unit& r, unsigned u) {
         if constexpr (ROWS)
@@ -180,8 +185,9 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
     Unit r;
     if (w < units) load(r, w);
     if constexpr (ROWS) {
-        if (p.K % 8 == 0) quantize(std::integral_constant<int, 4>{}, std::true_type{});
-        else quantize(std::integral_constant<int, 2>{}, std::false_type{});
+        if (p.K % 512 == 0) quantize(std::integral_constant<int, 0>{});
+        else if (p.K % 8 == 0) quantize(std::integral_constant<int, 1>{});
+        else quantize(std::integral_constant<int, 2>{});
         __syncthreads();
     }
     for (unsigned u = w; u < units; u += W) {
@@ -543,8 +549,8 @@ MmKind mm_choose(int M, int N, int K, double& us) {
 double rows_time(int M, int N, int K, int tn) {
     const double k = K, pieces = (double)(((M < 16 ? M : 16) * (long long)mx_scale_tiles(K) + 7) / 8);
     const double per_cu = (double)mx_row_tiles(M) * (double)((mx_row_tiles(N) + tn - 1) / tn) / num_cus();
-    return tile_time(2.96 + 0.034 * tn + (0.91e-4 * tn - 0.51e-4) * k + 0.265 * pieces, 2.3 + 0.2 * pieces,
-                     0.42 + 0.124 * tn + (1.44e-4 + 0.91e-4 * tn) * k + 0.1 * pieces, per_cu);
+    return tile_time(3.05 + 0.037 * tn + (0.94e-4 * tn - 0.77e-4) * k + 0.167 * pieces, 2.4 + 0.13 * pieces,
+                     0.42 + 0.132 * tn + (1.32e-4 + 0.78e-4 * tn) * k + 0.074 * pieces, per_cu);
 }
 
 }  // namespace
@@ -569,12 +575,12 @@ bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_
            int N, void* C, int act, hipStream_t s) {
     if (K > 0 && few_lds<float, 1, 4, 8>(K) <= 160 * 1024) {
         // One launch, in which every workgroup quantizes its 16 rows, or two, of which the
-        // first takes 2.5 us and its traffic at 4 TB/s?  Measured, us: 16 x 2048 x 2048 5.0 and
-        // 5.1, 16 x 2048 x 4096 7.2 and 5.4; 333 x 512 x 1024 4.5 and 6.9, 333 x 2048 x 2048
-        // 11.4 and 8.7.
+        // first takes 2.45 us and its traffic at 4.5 TB/s?  Measured, us: 16 x 2048 x 2048 4.4
+        // and 5.0, 16 x 2048 x 8192 9.0 and 6.1; 128 x 2048 x 1024 4.3 and 5.7, 333 x 2048 x
+        // 2048 10.1 and 8.2.
         double two, one = rows_time(M, N, K, 1);
         (void)mm_choose(M, N, K, two);
-        two += 2.5 + (double)M * K * (type_size(type) + 0.53) * 0.25e-6;
+        two += 2.45 + (double)M * K * (type_size(type) + 0.53) * 0.22e-6;
         int tn = 1;
         for (int n = 2; n <= 4; n *= 2)
             if (rows_time(M, N, K, n) < one) one = rows_time(M, N, K, tn = n);

@@ -169,6 +169,14 @@ def test_gemm(gpu, rng, M, N, K, t):
     _check_product(got, layers.mx_decode(*a, K), layers.mx_decode(*b, K), bias, act, t)
 
 
+@pytest.mark.parametrize("M,N,K", [(512, 2048, 4096), (512, 1111, 700), (1000, 600, 2048), (500, 2000, 4000)])
+def test_gemm_middle(gpu, rng, M, N, K):
+    a, b = _operand(rng, M, K), _operand(rng, N, K)
+    bias = rng.standard_normal(N).astype(np.float32)
+    got = _gemm(gpu, a, b, bias, 1, "bf16", M, N, K)
+    _check_product(got, layers.mx_decode(*a, K), layers.mx_decode(*b, K), bias, 1, "bf16")
+
+
 @pytest.mark.parametrize("t,M,N,K", [("f32", 3600, 4100, 200), ("bf16", 3585, 4097, 1), ("f16", 4096, 4096, 513),
                                      ("bf16", 20000, 1000, 700)])
 def test_gemm_large(gpu, rng, M, N, K, t):
@@ -192,6 +200,17 @@ def test_gemm_bad_blocks(gpu, rng, M, N, K):
     assert np.array_equal(bad, want) and np.array_equal(np.isnan(got), want)
 
 
+@pytest.mark.parametrize("M,N,K", [(3, 40, 100), (1000, 2500, 300)])
+def test_gemm_relu_nan(gpu, rng, M, N, K):
+    """ReLU keeps NaN, as the product without it gives it."""
+    a, b = _operand(rng, M, K), _operand(rng, N, K)
+    a[1][M // 2, 0] = 255
+    got = _gemm(gpu, a, b, None, 1, "f32", M, N, K)
+    want = np.zeros((M, N), bool)
+    want[M // 2] = True
+    assert np.array_equal(np.isnan(got), want) and (got[~want] >= 0).all()
+
+
 @pytest.mark.parametrize("M,N", [(1, 7), (40, 300), (300, 300)])
 def test_gemm_no_k(gpu, rng, M, N):
     """K = 0: the bias alone; no operand is read."""
@@ -213,8 +232,14 @@ FC = [(1, 64, 32), (1, 4096, 4096), (2, 130, 1), (7, 100, 1000), (16, 2053, 777)
       (100, 999, 513), (333, 2053, 1000), (600, 700, 2048), (1, 10, 8192), (5, 3000, 31)]
 
 
+# rows quantized in the product's launch (tiles of 16, 32 and 64 columns, K that is
+# whole pieces of 512, that ends between lanes and inside one) and in one before it
+FC_MORE = [(1, 8192, 512), (128, 2048, 512), (33, 2053, 1000), (16, 64, 1024), (4, 40, 20000), (130, 2100, 510),
+           (17, 3000, 520), (20, 300, 16), (64, 4100, 1536), (5, 8200, 2047), (16, 200, 8192), (300, 900, 3000)]
+
+
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("M,N,K", FC)
+@pytest.mark.parametrize("M,N,K", FC + FC_MORE)
 def test_fc(gpu, rng, M, N, K, t):
     code, dt = TYPES[t]
     x = values(torch.as_tensor(rng.standard_normal((M, K)) * np.exp(rng.standard_normal(K))).to(dt))
