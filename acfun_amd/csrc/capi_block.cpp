@@ -29,6 +29,15 @@ struct Checks {
         need(p != nullptr, what);
         return need(!type_ok(t) || (uintptr_t)p % type_size(t) == 0, "a tensor is not aligned to its elements");
     }
+    // what is written is apart from what is read: workgroups read it at any time
+    Checks& apart(const void* out, size_t n, const void* in, size_t m) {
+        const uintptr_t o = (uintptr_t)out, i = (uintptr_t)in;
+        return need(!in || o + n <= i || i + m <= o, "a result overlaps an input");
+    }
+    // or it is the same buffer, of which every element is read before it is written
+    Checks& apart_or_same(const void* out, const void* in, size_t n) {
+        return out == in ? *this : apart(out, n, in, n);
+    }
     Checks& param(const float* p) { return need((uintptr_t)p % 4 == 0, "a parameter is not aligned to 4 bytes"); }
     Checks& held(const uint8_t* codes, const uint8_t* scales) {
         need(codes && scales, "codes or scales are NULL");
@@ -78,6 +87,10 @@ int acfun_dev_quantize_mxfp4(const void* x, int type, int rows, int K, int trans
     if (!c.type(type).need(rows >= 0 && K >= 0, "a size is negative").ok) return -1;
     if (rows == 0 || K == 0) return 0;
     if (!c.tensor(x, type, "x is NULL").held(codes, scales).ok) return -1;
+    const size_t n = (size_t)rows * K * type_size(type);
+    c.apart(codes, mx_code_bytes(rows, K), x, n).apart(scales, mx_scale_bytes(rows, K), x, n);
+    c.apart(codes, mx_code_bytes(rows, K), scales, mx_scale_bytes(rows, K));
+    if (!c.ok) return -1;
     return call(c.who, [&] { return mx_quantize(x, type, rows, K, trans, codes, scales, resolve(stream)); });
 }
 
@@ -87,6 +100,8 @@ int acfun_dev_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, int 
     if (!c.type(type).need(rows >= 0 && K >= 0, "a size is negative").ok) return -1;
     if (rows == 0 || K == 0) return 0;
     if (!c.tensor(x, type, "x is NULL").held(codes, scales).ok) return -1;
+    const size_t n = (size_t)rows * K * type_size(type);
+    if (!c.apart(x, n, codes, mx_code_bytes(rows, K)).apart(x, n, scales, mx_scale_bytes(rows, K)).ok) return -1;
     return call(c.who, [&] { return mx_dequantize(codes, scales, rows, K, x, type, resolve(stream)); });
 }
 
@@ -97,6 +112,12 @@ int acfun_dev_gemm_mxfp4(int M, int N, int K, const uint8_t* A, const uint8_t* a
     if (M == 0 || N == 0) return 0;
     if (K > 0) c.held(A, a_scales).held(B, b_scales);
     if (!c.tensor(C, type, "C is NULL").param(bias).ok) return -1;
+    const size_t n = (size_t)M * N * type_size(type);
+    if (K > 0) {
+        c.apart(C, n, A, mx_code_bytes(M, K)).apart(C, n, a_scales, mx_scale_bytes(M, K));
+        c.apart(C, n, B, mx_code_bytes(N, K)).apart(C, n, b_scales, mx_scale_bytes(N, K));
+    }
+    if (!c.apart(C, n, bias, 4 * (size_t)N).ok) return -1;
     return call(c.who, [&] {
         return mx_gemm(M, N, K, A, a_scales, B, b_scales, C, type, bias, act, resolve(stream));
     });
@@ -109,6 +130,12 @@ int acfun_dev_fc_mxfp4(const void* input, int type, int N, int Cin, const uint8_
     if (N == 0 || Cout == 0) return 0;
     if (Cin > 0) c.tensor(input, type, "input is NULL").held(weight, wscale);
     if (!c.tensor(output, type, "output is NULL").param(bias).ok) return -1;
+    const size_t n = (size_t)N * Cout * type_size(type);
+    if (Cin > 0) {
+        c.apart(output, n, input, (size_t)N * Cin * type_size(type));
+        c.apart(output, n, weight, mx_code_bytes(Cout, Cin)).apart(output, n, wscale, mx_scale_bytes(Cout, Cin));
+    }
+    if (!c.apart(output, n, bias, 4 * (size_t)Cout).ok) return -1;
     return call(c.who, [&] {
         return mx_fc(input, type, N, Cin, weight, wscale, bias, Cout, output, act, resolve(stream));
     });
@@ -153,6 +180,8 @@ int acfun_dev_norm(const void* x, int type, int rows, int cols, int kind, const 
     c.need(eps >= 0.f, "eps is negative");
     c.tensor(x, type, "x is NULL").tensor(h, type, "h is NULL").param(weight).param(bias);
     if (!c.ok) return -1;
+    const size_t n = (size_t)rows * cols * type_size(type), np = 4 * (size_t)cols;
+    if (!c.apart_or_same(h, x, n).apart(h, n, weight, np).apart(h, n, bias, np).ok) return -1;
     NormArgs a{nullptr, x, rows, cols, kind, nullptr, nullptr, nullptr, 1, 1.f, weight, bias, eps, nullptr, h};
     return call(c.who, [&] { return norm_rows(a, type, resolve(stream)); });
 }
@@ -173,6 +202,15 @@ int acfun_dev_norm_residual(const void* y, const void* x, int type, int rows, in
     if (h) c.tensor(h, type, "");
     c.param(post_w).param(post_b).param(pre_w).param(pre_b);
     c.need(h != x_out, "h and x_out are the same buffer");
+    if (!c.ok) return -1;
+    const size_t n = (size_t)rows * cols * type_size(type), np = 4 * (size_t)cols;
+    const size_t ng = gate ? ((size_t)rows + gate_group - 1) / gate_group * cols * type_size(type) : 0;
+    c.apart(x_out, n, h, h ? n : 0);
+    for (void* out : {x_out, h}) {
+        if (!out) continue;
+        c.apart_or_same(out, x, n).apart_or_same(out, y, n).apart(out, n, gate, ng);
+        for (const float* q : {post_w, post_b, pre_w, pre_b}) c.apart(out, n, q, np);
+    }
     if (!c.ok) return -1;
     NormArgs a{y, x, rows, cols, kind, post_w, post_b, gate, gate ? gate_group : 1, res_scale, pre_w, pre_b, eps,
                x_out, h};

@@ -58,6 +58,7 @@ struct MmArgs {
     void* C;
     const float* bias;
     int act, gm, gn;                // tiles of C
+    int rows = 0;                   // of LDS for quantized rows
 };
 
 // ---------------------------------------------------------------- few rows
@@ -66,27 +67,30 @@ struct MmArgs {
 // memory to registers, and so does A if X is void.  Otherwise A is float rows of X,
 // which the workgroup quantizes into LDS for its tile, while B's first loads are on
 // their way.
-template <class X, int TM, int TN, int W>
-__host__ __device__ inline size_t few_lds(int K) {
-    return (size_t)W * TM * TN * 68 * 16 + (std::is_void_v<X> ? 0 : (size_t)TM * mx_scale_tiles(K) * (4096 + 256));
-}
+template <int TM, int TN, int W>
+constexpr size_t kFewSums = (size_t)W * TM * TN * 68 * 16;
+// The LDS of quantized rows: room for 1, 2, 4, 8 or 16 of them.
+inline int few_rows(int M) { return M > 8 ? 16 : M > 4 ? 8 : M > 2 ? 4 : M; }
+inline size_t few_rows_lds(int M, int K) { return (size_t)few_rows(M) * mx_scale_tiles(K) * (256 + 16); }
 
 template <class T, class X, int TM, int TN, int W, int U>
 __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
     constexpr bool ROWS = !std::is_void_v<X>;
     using E = std::conditional_t<ROWS, X, float>;
+    static_assert(!ROWS || TM == 1, "rows of one tile are quantized");
     // partial sums: 16 lanes' quads, and one more, so that the threads of a row read 16
     // different banks; then the quantized rows: codes, scales
     extern __shared__ __attribute__((aligned(16))) char smx[];
     f4v(*const red)[TM * TN][68] = (f4v(*)[TM * TN][68])smx;
-    char* const rc = smx + W * TM * TN * 68 * 16;
+    char* const rc = smx + kFewSums<TM, TN, W>;
+    const unsigned R = p.rows;                                  // room for rows, a power of two
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned total = (unsigned)p.gm * p.gn, L = xcd_tile(total);
     if (L >= total) return;
     const unsigned tn = p.gm == 1 ? L : L / p.gm, tm = L - tn * p.gm;
     const unsigned kt = mx_k_tiles(p.K), st = mx_scale_tiles(p.K), units = (kt + U - 1) / U;
     const unsigned mt = (unsigned)mx_row_tiles(p.M) - 1, nt = (unsigned)mx_row_tiles(p.N) - 1;
-    char* const rs = rc + TM * st * 4096;
+    char* const rs = rc + st * 256 * R;
     const uint8_t *a[TM], *as[TM], *b[TN], *bs[TN];             // (uniform)
     if constexpr (!ROWS)
 #pragma unroll
@@ -101,7 +105,8 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
         b[i] = p.B + ((uint64_t)t * kt << 10);
         bs[i] = p.Bs + ((uint64_t)t * st << 8);
     }
-    const unsigned o16 = lane * 16u, o4 = lane * 4u, oq = (lane ^ (lane >> 4)) * 16u;
+    const unsigned o16 = lane * 16u, o4 = lane * 4u, j16 = lane >> 4, l16 = lane & 15;
+    const unsigned oq = (j16 * R + ((l16 ^ j16) & (R - 1))) * 16, os = (j16 * R + (l16 & (R - 1))) * 4;
     f4v acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -131,25 +136,26 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
     // Pieces of a row and 512 k, eight values to a lane; four to a wave at once, for the
     // latency of their loads, then one by one.  ENDS: 0 where K is whole pieces, 1 where
     // it ends between lanes, 2 inside a lane's eight values (a kernel fetches its code
-    // as it goes, so each has its own).  Rows past M are left as they are, for rows of C
-    // that are not stored.  Codes lie as in an operand but for the place of row r in block
-    // j of the s-th 128 k, which is r ^ (4 s + j): a piece's blocks are written to
-    // different banks.
+    // as it goes, so each has its own).  Codes and scales lie as in an operand but for the
+    // room, which is for R rows instead of 16, and for the place of row r's codes in
+    // block j of the s-th 128 k, which is r ^ (4 s + j): a piece's blocks are written to
+    // different banks.  Rows past M are whatever lies there, for rows of C that are not
+    // stored.
     auto quantize = [&](auto ENDS) {
         constexpr int ends = decltype(ENDS)::value;
-        const unsigned rows = (unsigned)p.M - tm * (16 * TM) < 16 * TM ? p.M - tm * (16 * TM) : 16 * TM;
+        const unsigned rows = (unsigned)p.M - tm * 16 < 16 ? p.M - tm * 16 : 16;
         const unsigned du = W / rows, dm = W % rows;            // from a wave's piece to its next
         unsigned u = w / rows, m = w - u * rows;
         const unsigned j = (lane >> 2) & 3, s = lane >> 4, part = lane & 3;
-        const E* const x = (const E*)p.A + (uint64_t)tm * (16 * TM) * (unsigned)p.K;
+        const E* const x = (const E*)p.A + (uint64_t)tm * 16 * (unsigned)p.K;
         auto some = [&](auto QC) {
             constexpr int Q = decltype(QC)::value;
             typename VecOf<E, 8>::type v[Q] = {};
             unsigned to[Q], row[Q];
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
-                to[i] = (TM == 1 ? u : (m >> 4) * st + u) * 256;
-                row[i] = m & 15;
+                to[i] = u * 16 * R;
+                row[i] = m;
                 const E* const from = x + (uint64_t)m * (unsigned)p.K + 512ull * u;
                 const int left = p.K - (int)(512 * u) - 8 * lane;
                 if constexpr (ends == 2) v[i] = load_vec<E, 8>(from + 8u * lane, left);
@@ -161,9 +167,10 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
             for (int i = 0; i < Q; ++i) {
                 unsigned byte;
                 const unsigned c = mx_codes_of4(v[i], byte);
-                *(unsigned*)(rc + to[i] * 16 + s * 1024 + j * 256 + (row[i] ^ (4 * s + j)) * 16 + 4 * part) = c;
+                const unsigned block = (4 * s + j) * R + ((row[i] ^ (4 * s + j)) & (R - 1));
+                *(unsigned*)(rc + (to[i] + block) * 16 + 4 * part) = c;
                 // (all four lanes of a block have its scale byte)
-                rs[to[i] + 64 * j + 4 * row[i] + s] = (char)byte;
+                rs[to[i] + (j * R + row[i]) * 4 + s] = (char)byte;
             }
         };
         const unsigned mine = (rows * st + W - 1 - w) / W;
@@ -173,14 +180,14 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
         for (; n < mine; ++n) some(std::integral_constant<int, 1>{});
     };
     auto take_rows = [&](Unit& r, unsigned u) {
-        if constexpr (ROWS)
+        if constexpr (ROWS) {
 #pragma unroll
-            for (int j = 0; j < TM; ++j) {
-#pragma unroll
-                for (int i = 0; i < U; ++i)
-                    r.a[i][j] = *(const i4v*)(rc + (j * st * 4 + u * U + i) * 1024 + (oq ^ ((u * U + i) & 3) * 64));
-                r.sa[j] = *(const unsigned*)(rs + (j * st + (u * U >> 2)) * 256 + o4);
+            for (int i = 0; i < U; ++i) {
+                const unsigned t = u * U + i;
+                r.a[i][0] = *(const i4v*)(rc + t * 64 * R + (oq ^ ((t & 3) * 64 & (R - 1) * 16)));
             }
+            r.sa[0] = *(const unsigned*)(rs + (u * U >> 2) * 16 * R + os);
+        }
     };
     Unit r;
     if (w < units) load(r, w);
@@ -476,13 +483,14 @@ bool launch_few(MmArgs a, hipStream_t s) {
     (void)attr;
     a.gm = (int)((mx_row_tiles(a.M) + TM - 1) / TM);
     a.gn = (int)((mx_row_tiles(a.N) + TN - 1) / TN);
+    a.rows = few_rows(a.M);
     const long long grid = ((long long)a.gm * a.gn + 7) / 8 * 8;
     if (grid >= (1ll << 31)) {
         set_error("acfun_dev_gemm_mxfp4: too large");
         return false;
     }
     ACFUN_LAUNCH("k_mxmm_few", (k_mxmm_few<T, X, TM, TN, W, U>), dim3((unsigned)grid), dim3(64 * W),
-                 (few_lds<X, TM, TN, W>(a.K)), s, a);
+                 (kFewSums<TM, TN, W> + (std::is_void_v<X> ? 0 : few_rows_lds(a.M, a.K))), s, a);
     return check_launch("k_mxmm_few");
 }
 
@@ -546,7 +554,9 @@ MmKind mm_choose(int M, int N, int K, double& us) {
 
 // The same for a layer whose workgroups each quantize their 16 rows, with tiles of 16,
 // 32 or 64 columns (tn tiles of 16): `pieces` of a row and 512 k fall to each wave.
+// Where LDS has no room for the rows it cannot be done.
 double rows_time(int M, int N, int K, int tn) {
+    if (kFewSums<1, 1, 8> * tn + few_rows_lds(M, K) > 160 * 1024) return 1e30;
     const double k = K, pieces = (double)(((M < 16 ? M : 16) * (long long)mx_scale_tiles(K) + 7) / 8);
     const double per_cu = (double)mx_row_tiles(M) * (double)((mx_row_tiles(N) + tn - 1) / tn) / num_cus();
     return tile_time(3.05 + 0.037 * tn + (0.94e-4 * tn - 0.77e-4) * k + 0.167 * pieces, 2.4 + 0.13 * pieces,
@@ -573,7 +583,7 @@ bool mx_gemm(int M, int N, int K, const uint8_t* A, const uint8_t* As, const uin
 
 bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_t* Bs, const float* bias,
            int N, void* C, int act, hipStream_t s) {
-    if (K > 0 && few_lds<float, 1, 4, 8>(K) <= 160 * 1024) {
+    if (K > 0) {
         // One launch, in which every workgroup quantizes its 16 rows, or two, of which the
         // first takes 2.45 us and its traffic at 4.5 TB/s?  Measured, us: 16 x 2048 x 2048 4.4
         // and 5.0, 16 x 2048 x 8192 9.0 and 6.1; 128 x 2048 x 1024 4.3 and 5.7, 333 x 2048 x
@@ -593,6 +603,14 @@ bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_
                 return launch_few<T, T, 1, 4, 8, 2>(a, s);
             });
         }
+    }
+    // a graph would keep the addresses of temporaries that go back to the pool here
+    hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
+    if (K > 0 && !check(hipStreamIsCapturing(s, &captured), "hipStreamIsCapturing")) return false;
+    if (captured != hipStreamCaptureStatusNone) {
+        set_error("acfun_dev_fc_mxfp4: these sizes need temporaries, which a graph cannot keep: capture "
+                  "acfun_dev_quantize_mxfp4 and acfun_dev_gemm_mxfp4 with buffers of the caller's");
+        return false;
     }
     Scratch codes(mx_code_bytes(M, K), s), scales(mx_scale_bytes(M, K), s);
     if (K > 0 && (!codes.p || !scales.p)) return false;

@@ -252,7 +252,8 @@ int acfun_dev_softmax(const float* input, int rows, int cols, float* output, voi
  * held in fp32 and a result is rounded to its type once, when it is stored.
  * The acfun_dev_* calls take device pointers and a stream as above; they return
  * 0, or -1 with acfun_last_error() and nothing queued: on a negative size, an
- * unknown type or code, a NULL or misaligned pointer.  An empty output is 0. */
+ * unknown type or code, a NULL or misaligned pointer, a result that overlaps an
+ * input (but where a call says that it may be one).  An empty output is 0. */
 #define ACFUN_F32 0
 #define ACFUN_BF16 1
 #define ACFUN_F16 2
@@ -288,7 +289,10 @@ int acfun_dev_gemm_mxfp4(int M, int N, int K, const uint8_t* A, const uint8_t* a
                          const float* bias, int act, void* stream);
 /* A fully connected layer with weights held in MXFP4 (an operand of Cout rows):
  * input [N, Cin] is quantized as acfun_dev_quantize_mxfp4 does and multiplied;
- * output [N, Cout].  Input and output are of `type`. */
+ * output [N, Cout].  Input and output are of `type`.  Small layers are one launch
+ * without temporaries; for others the quantized input lies in the library's pool, and
+ * a call on a stream that is being captured into a graph is refused: quantize into
+ * buffers of the caller's and multiply, which is the same.  */
 int acfun_dev_fc_mxfp4(const void* input, int type, int N, int Cin, const uint8_t* weight,
                        const uint8_t* wscale, const float* bias, int Cout, void* output, int act,
                        void* stream);

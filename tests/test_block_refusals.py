@@ -130,3 +130,57 @@ def test_oracle_codes():
                 near = np.flatnonzero(d == d.min())
                 k = near[0] if len(near) == 1 else [n for n in near if n % 2 == 0][0]
                 assert v[r, 32 * b + i] == np.sign(blk[i]) * grid[k]
+
+
+def test_overlaps():
+    """A result that overlaps an input, by its first or last bytes."""
+    L = capi.lib()
+    n = 4 * 64 * 4                                           # bytes of a 4 x 64 fp32 tensor
+    far = [P + (i << 16) for i in range(8)]
+    nc = L.acfun_mxfp4_code_bytes(4, 64)
+    word = "overlaps"
+
+    def quant(x=far[0], c=far[1], s=far[2]):
+        return L.acfun_dev_quantize_mxfp4(x, 0, 4, 64, 0, c, s, None)
+
+    def dequant(x=far[0], c=far[1], s=far[2]):
+        return L.acfun_dev_dequantize_mxfp4(c, s, 4, 64, x, 0, None)
+    for f in (quant, dequant):
+        _refused(f(x=far[1]), word)
+        _refused(f(x=far[1] + nc - 16), word)
+        _refused(f(x=far[2] - n + 16), word)
+    _refused(quant(s=far[1] + nc - 16), word)
+
+    def gemm(c, bias=None):
+        return L.acfun_dev_gemm_mxfp4(4, 64, 64, far[0], far[1], far[2], far[3], c, 0, bias, 0, None)
+    for i in range(4):
+        _refused(gemm(far[i] + 4), word)
+        _refused(gemm(far[i] - n + 4), word)
+    _refused(gemm(far[5], far[5] + n - 4), word)
+
+    def fc(c, bias=None):
+        return L.acfun_dev_fc_mxfp4(far[0], 0, 4, 64, far[1], far[2], bias, 64, c, 0, None)
+    for i in range(3):
+        _refused(fc(far[i]), word)
+        _refused(fc(far[i] - n + 4), word)
+    _refused(fc(far[5], far[5]), word)
+
+    def norm(h, w=far[1], b=far[2]):
+        return L.acfun_dev_norm(far[0], 0, 4, 64, 1, w, b, 1e-5, h, None)
+    _refused(norm(far[0] + 4), word)
+    _refused(norm(far[0] - n + 4), word)
+    _refused(norm(far[1]), word)
+    _refused(norm(far[2] - n + 4), word)
+
+    def res(xo=far[2], h=far[3], gate=far[4], group=4):
+        return L.acfun_dev_norm_residual(far[0], far[1], 0, 4, 64, 0, far[5], None, gate, group, 1.0, far[6],
+                                         None, 1e-5, xo, h, None)
+    for i in range(2):
+        _refused(res(xo=far[i] + 4), word)
+        _refused(res(h=far[i] - n + 4), word)
+    _refused(res(h=far[2] + n - 4), word)
+    _refused(res(xo=far[4]), word)
+    _refused(res(h=far[4] - n + 4), word)
+    _refused(res(xo=far[4] + n - 4, group=1), word)
+    _refused(res(xo=far[5]), word)
+    _refused(res(h=far[6] + 4), word)

@@ -235,7 +235,8 @@ FC = [(1, 64, 32), (1, 4096, 4096), (2, 130, 1), (7, 100, 1000), (16, 2053, 777)
 # rows quantized in the product's launch (tiles of 16, 32 and 64 columns, K that is
 # whole pieces of 512, that ends between lanes and inside one) and in one before it
 FC_MORE = [(1, 8192, 512), (128, 2048, 512), (33, 2053, 1000), (16, 64, 1024), (4, 40, 20000), (130, 2100, 510),
-           (17, 3000, 520), (20, 300, 16), (64, 4100, 1536), (5, 8200, 2047), (16, 200, 8192), (300, 900, 3000)]
+           (17, 3000, 520), (20, 300, 16), (64, 4100, 1536), (5, 8200, 2047), (16, 200, 8192), (300, 900, 3000),
+           (1, 30, 40000), (2, 30, 33000), (3, 50, 20000), (8, 40, 17000), (16, 40, 17408), (7, 600, 1500)]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -328,3 +329,43 @@ def test_repeats_and_graph(gpu, rng, M, N, K):
             call()
             s.synchronize()
             assert torch.equal(out, first), i
+
+
+def test_graph_of_many_rows(gpu, rng):
+    """A layer that needs temporaries is refused while its stream is captured, with the
+    capture left whole; quantizing into the caller's buffers and multiplying is captured
+    and gives the layer's bits."""
+    M, N, K = 600, 2000, 2000
+    b = _operand(rng, N, K)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        x = torch.as_tensor(rng.standard_normal((M, K)), dtype=torch.bfloat16).cuda()
+        d = [torch.as_tensor(v).cuda() for v in layers.mx_tiles(*b)]
+        c = torch.empty(gpu.acfun_mxfp4_code_bytes(M, K), dtype=torch.uint8, device="cuda")
+        sc = torch.empty(gpu.acfun_mxfp4_scale_bytes(M, K), dtype=torch.uint8, device="cuda")
+        want, out = (torch.zeros((M, N), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+
+        def fc(y):
+            return gpu.acfun_dev_fc_mxfp4(x.data_ptr(), 1, M, K, d[0].data_ptr(), d[1].data_ptr(), None, N,
+                                          y.data_ptr(), 0, s.cuda_stream)
+
+        def parts():
+            assert gpu.acfun_dev_quantize_mxfp4(x.data_ptr(), 1, M, K, 0, c.data_ptr(), sc.data_ptr(),
+                                                s.cuda_stream) == 0, capi.last_error()
+            assert gpu.acfun_dev_gemm_mxfp4(M, N, K, c.data_ptr(), sc.data_ptr(), d[0].data_ptr(),
+                                            d[1].data_ptr(), out.data_ptr(), 1, None, 0,
+                                            s.cuda_stream) == 0, capi.last_error()
+        assert fc(want) == 0, capi.last_error()
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            refused = fc(out), capi.last_error()
+            parts()
+        assert refused[0] == -1 and "temporaries" in refused[1]
+        for i in range(3):
+            out.zero_()
+            g.replay()
+            s.synchronize()
+            assert torch.equal(out, want), i
+            assert fc(out) == 0                              # other work between the replays
+            s.synchronize()
