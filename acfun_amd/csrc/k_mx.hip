@@ -109,7 +109,8 @@ __global__ __launch_bounds__(256) void k_mx_dequant(const uint8_t* __restrict__ 
         pair(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s], scale, 1));
         pair(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s], scale, 2));
         pair(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s], scale, 3));
-        if (k < left) store_vec<T, 8>(xr + k, left - k, f);
+        // (a lane's eight fp32 values are two stores of half lines, which the caches join)
+        if (k < left) store_vec<T, 8, sizeof(T) == 2>(xr + k, left - k, f);
     }
 }
 

@@ -462,7 +462,7 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void k_mxmm(MmArgs p) {
         if (left == CV)
 #pragma unroll 8
             for (int r = lane / LPR; r < rows; r += RPI)
-                *(tvu*)(C + (size_t)r * p.N + cl) = *(const tv*)(slab + r * RS + cl);
+                __builtin_nontemporal_store(*(const tv*)(slab + r * RS + cl), (tvu*)(C + (size_t)r * p.N + cl));
         else if (left > 0)                                  // the last columns
 #pragma unroll 1
             for (int r = lane / LPR; r < rows; r += RPI)

@@ -87,7 +87,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
     };
     auto put = [&](T* p, int i, const float (&v)[VN]) {
         if constexpr (!WHOLE) store_vec<T, VN>(p + col(i), cols - col(i), v);
-        else if (col(i) < cols) store_vec<T, VN>(p + col(i), VN, v);
+        else if (col(i) < cols) store_vec<T, VN, true>(p + col(i), VN, v);
     };
     V yv[CH], xv[CH], gv[KEEP ? CH : 1];           // a row of x beside y: KEEP only
     int group = -1;

@@ -55,13 +55,17 @@ __device__ __forceinline__ typename VecOf<T, N>::type load_vec(const T* p, int l
     for (int e = 0; e < N; ++e) v[e] = e < left ? p[e] : (T)fill;
     return v;
 }
-template <class T, int N>
+// The first `left` of N values to p.  PAST: past the caches, for results that a kernel
+// writes as whole lines and that would push out what others read.
+template <class T, int N, bool PAST = false>
 __device__ __forceinline__ void store_vec(T* p, int left, const float (&v)[N]) {
     if (left >= N) {
-        typename VecOf<T, N>::type o;
+        typedef typename VecOf<T, N>::type V;
+        V o;
 #pragma unroll
         for (int e = 0; e < N; ++e) o[e] = (T)v[e];
-        *(typename VecOf<T, N>::type*)p = o;
+        if constexpr (PAST) __builtin_nontemporal_store(o, (V*)p);
+        else *(V*)p = o;
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
