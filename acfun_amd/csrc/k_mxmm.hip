@@ -3,17 +3,20 @@
 // The weights are the MFMA's A operand, so a lane's consecutive results are
 // consecutive columns of one row of C.
 //
-// k_mxmm_few: small tiles, K split between a workgroup's waves.  Latency and the
-// reading of the weights bound it.  1 x 4096 x 4096: 4.4 us with the quantization of
-// its row; 128 x 8192 x 4096: 9.1 us.
+// k_mxmm_few: tiles of 16, 32 or 64 on the 16 x 16 x 128 MFMA, K split between a
+// workgroup's waves.  A launch's latency bounds the smallest, the reading of the weights
+// the others: 1 x 4096 x 4096 3.5 us in a graph with the quantization of its row, 1 x
+// 16384 -> 4096 8.4 (34 MB, 4 TB/s), 128 x 8192 x 4096 6.8.
 //
 // k_mxmm: four waves of 2 x 2 or 4 x 4 blocks of 32 x 32, operands DMA'd into LDS in
 // chunks of 128 k, four stages.  The 256 x 256 tile needs 512 bytes of LDS reads per
 // MFMA, half of what 128 x 128 does.  Its loop takes 1,240 cycles a chunk, of which
 // the MFMAs are 1,024; random data at that rate brings the clock down to 1.5 GHz
-// (MFMAs alone, on registers, reach 6.5 PFLOP/s with them and 9.4 on zeros).
-// 8192^3 bf16: 250 us (4.4 PFLOP/s); 4096^3 to fp32: 40 us (3.4); with a wave to each
-// 16 x 16 of C and operands from memory 1,800 and 190.
+// (MFMAs alone, on registers, reach 6.5 PFLOP/s with them and 9.4 on zeros), and
+// without its LDS reads, or without its DMA, the kernel would be 6 or 10 % faster.
+// 8192^3 bf16: 242 us (4.5 PFLOP/s); 4096^3 to fp32: 40 us (3.4; one tile for each CU, so
+// that its 67 MB of results are stored at once, at the end); with a wave to each 16 x
+// 16 of C and operands from memory 1,800 and 190.
 #include <type_traits>
 #include <utility>
 
@@ -516,12 +519,12 @@ bool launch_many(MmArgs a, hipStream_t s) {
 }
 
 // Times in us that choose a kernel and its tile, fitted to those of every tile over
-// 518 sizes (M of 16 to 8192, N of 64 to 8192, K of 128 to 8192; bf16, replayed from a
+// 546 sizes (M of 16 to 8192, N of 64 to 8192, K of 128 to 8192; bf16, replayed from a
 // graph): a call takes `lat` while the CUs have less than a tile each, and `base` and
-// `each` times the tiles of a CU from there.  The tile chosen is 1.4 % slower than the
+// `each` times the tiles of a CU from there.  The tile chosen is 0.8 % slower than the
 // best of each size in the mean.  Measured, us: 128 x 8192 x 4096 9.7 with tiles of 32,
 // 6.8 with 64, 11.3 with 128; 512 x 8192 x 1024 15 with 64, 7.1 with 128; 2048 x 8192 x
-// 4096 45 with 128, 39 with 256.
+// 4096 45 with 128, 38 with 256.
 double tile_time(double lat, double base, double each, double tiles_per_cu) {
     const double t = base + each * tiles_per_cu;
     return t > lat ? t : lat;
@@ -537,11 +540,11 @@ MmKind mm_choose(int M, int N, int K, double& us) {
     };
     auto more = [](double a, double b) { return a > b ? a : b; };
     const double t[KINDS] = {
-        tile_time(2.78 + 0.75e-4 * k, 2.1 + 1.2e-4 * k, 0.42 + 1.6e-4 * k, per_cu(16)),
-        tile_time(2.8 + 3.0e-4 * k, 2.65 + 3.2e-4 * k, more(0.28 + 2.75e-4 * k, 3.8e-4 * k), per_cu(32)),
-        tile_time(3.85 + 8.0e-4 * k, 2.15 + 2.9e-4 * k, 2.4 + 8.5e-4 * k, per_cu(64)),
-        tile_time(3.9 + 17.2e-4 * k, 3.6 + 3.3e-4 * k, more(1.9 + 17.8e-4 * k, 20.7e-4 * k), per_cu(128)),
-        tile_time(7.05 + 45.2e-4 * k, 6.0, more(7.0 + 61.7e-4 * k, 72.7e-4 * k), per_cu(256)),
+        tile_time(2.72 + 0.91e-4 * k, 2.05 + 1.1e-4 * k, 0.417 + 1.55e-4 * k, per_cu(16)),
+        tile_time(0.8 + 5.5e-4 * k, 2.76 + 2.8e-4 * k, more(0.235 + 2.0e-4 * k, 4.0e-4 * k), per_cu(32)),
+        tile_time(3.81 + 7.9e-4 * k, 2.05 + 2.9e-4 * k, 2.41 + 8.7e-4 * k, per_cu(64)),
+        tile_time(3.89 + 17.2e-4 * k, 3.79 + 4.4e-4 * k, 1.51 + 19.8e-4 * k, per_cu(128)),
+        tile_time(7.36 + 43.7e-4 * k, 3.73, more(8.04 + 67.6e-4 * k, 77.4e-4 * k), per_cu(256)),
     };
     // 32-bit offsets into a tile's operands
     const int kinds = K > 0 && K <= (1 << 22) ? KINDS : MANY128;
