@@ -533,8 +533,8 @@ double tile_time(double lat, double base, double each, double tiles_per_cu) {
 enum MmKind { FEW16, FEW32, FEW64, MANY128, MANY256, KINDS };
 
 // The fastest kernel for a product, and its time.
-MmKind mm_choose(int M, int N, int K, double& us) {
-    const double cus = num_cus(), k = K;
+MmKind mm_choose(int M, int N, int K, double cus, double& us) {
+    const double k = K;
     auto per_cu = [&](int b) {
         return (double)(((long long)M + b - 1) / b) * (double)(((long long)N + b - 1) / b) / cus;
     };
@@ -558,10 +558,10 @@ MmKind mm_choose(int M, int N, int K, double& us) {
 // The same for a layer whose workgroups each quantize their 16 rows, with tiles of 16,
 // 32 or 64 columns (tn tiles of 16): `pieces` of a row and 512 k fall to each wave.
 // Where LDS has no room for the rows it cannot be done.
-double rows_time(int M, int N, int K, int tn) {
+double rows_time(int M, int N, int K, double cus, int tn) {
     if (kFewSums<1, 1, 8> * tn + few_rows_lds(M, K) > 160 * 1024) return 1e30;
     const double k = K, pieces = (double)(((M < 16 ? M : 16) * (long long)mx_scale_tiles(K) + 7) / 8);
-    const double per_cu = (double)mx_row_tiles(M) * (double)((mx_row_tiles(N) + tn - 1) / tn) / num_cus();
+    const double per_cu = (double)mx_row_tiles(M) * (double)((mx_row_tiles(N) + tn - 1) / tn) / cus;
     return tile_time(3.05 + 0.037 * tn + (0.94e-4 * tn - 0.77e-4) * k + 0.167 * pieces, 2.4 + 0.13 * pieces,
                      0.42 + 0.132 * tn + (1.32e-4 + 0.78e-4 * tn) * k + 0.074 * pieces, per_cu);
 }
@@ -574,7 +574,7 @@ bool mx_gemm(int M, int N, int K, const uint8_t* A, const uint8_t* As, const uin
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         double us;
-        switch (mm_choose(M, N, K, us)) {
+        switch (mm_choose(M, N, K, num_cus(), us)) {
             case FEW16: return launch_few<T, void, 1, 1, 8, 4>(a, s);
             case FEW32: return launch_few<T, void, 2, 2, 4, 2>(a, s);
             case FEW64: return launch_few<T, void, 4, 4, 8, 1>(a, s);
@@ -591,12 +591,13 @@ bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_
         // first takes 2.45 us and its traffic at 4.5 TB/s?  Measured, us: 16 x 2048 x 2048 4.4
         // and 5.0, 16 x 2048 x 8192 9.0 and 6.1; 128 x 2048 x 1024 4.3 and 5.7, 333 x 2048 x
         // 2048 10.1 and 8.2.
-        double two, one = rows_time(M, N, K, 1);
-        (void)mm_choose(M, N, K, two);
+        const double cus = num_cus();
+        double two, one = rows_time(M, N, K, cus, 1);
+        (void)mm_choose(M, N, K, cus, two);
         two += 2.45 + (double)M * K * (type_size(type) + 0.53) * 0.22e-6;
         int tn = 1;
         for (int n = 2; n <= 4; n *= 2)
-            if (rows_time(M, N, K, n) < one) one = rows_time(M, N, K, tn = n);
+            if (const double t = rows_time(M, N, K, cus, n); t < one) one = t, tn = n;
         if (one < two) {
             const MmArgs a{M, N, K, x, nullptr, B, Bs, C, bias, act, 0, 0};
             return with_type(type, [&](auto t) {

@@ -9,10 +9,12 @@
 // is the norm of the sum before its rounding).
 //
 // Memory bounds it: a row is read and written once, whatever the statistics
-// need.  Measured: norm and residual of 8192 x 8192 bf16 102 us (537 MB, 5.24
-// TB/s; a copy reaches 5.55), the norm of 4096 x 4096 fp16 13.9 us; one token 4.7
-// and 4.9 us, of which the launch is most.  With a value per thread and step
-// and parameters read for every row: 478, 26.1, 5.6 and 21.2.
+// need, and results of whole lines are stored past the caches.  Measured: norm and
+// residual of 8192 x 8192 bf16 97 us (537 MB, 5.5 TB/s, a copy's rate), the norm of
+// 4096 x 4096 fp16 12.3 us; one token 2.1 and eight 3.9 us in a graph, 4.1 and 4.7 from
+// the host, which is the cost of a launch.  Rows whose width is no whole chunk start
+// off a dword's boundary in 16-bit types: 8192 x 8111 135 us.  With a value per thread
+// and step and parameters read for every row: 478, 26.1, 5.6 and 21.2.
 #include <type_traits>
 
 #include "mx.hpp"
@@ -225,10 +227,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void k_norm_row(NormArgs 
 }
 
 template <class T, int TPR, int CH>
-bool launch(NormArgs a, hipStream_t s) {
+bool launch(NormArgs a, int cus, hipStream_t s) {
     constexpr int RPB = TPR == 64 ? 4 : 1, THREADS = TPR < 256 ? 256 : TPR;
     // at most four waves per SIMD, and as many rows to each workgroup
-    const long long groups = ((long long)a.rows + RPB - 1) / RPB, most = num_cus() * (1024 / THREADS);
+    const long long groups = ((long long)a.rows + RPB - 1) / RPB, most = cus * (1024 / THREADS);
     const long long each = (groups + most - 1) / most;
     const dim3 grid((unsigned)((groups + each - 1) / each)), block(THREADS);
     a.step = (int)(grid.x * RPB);
@@ -247,16 +249,19 @@ bool norm_rows(const NormArgs& a, int type, hipStream_t s) {
         using T = decltype(t);
         constexpr int VN = 16 / (int)sizeof(T);
         const int n = (a.cols + VN - 1) / VN;             // chunks of a row
-        // few rows: one chunk to a thread; many: two, and fewer waves to wait for
-        const bool few = a.rows <= num_cus();
-        if (n <= 64) return launch<T, 64, 1>(a, s);
-        if (n <= 128) return launch<T, 64, 2>(a, s);
-        if (n <= 256) return launch<T, 256, 1>(a, s);
-        if (n <= 512) return few ? launch<T, 512, 1>(a, s) : launch<T, 256, 2>(a, s);
-        if (n <= 1024) return few ? launch<T, 1024, 1>(a, s) : launch<T, 512, 2>(a, s);
-        if (n <= 2048) return launch<T, 1024, 2>(a, s);
-        if (n <= 4096) return launch<T, 1024, 4>(a, s);
-        if constexpr (VN == 4) return launch<T, 1024, 8>(a, s);
+        // Two chunks to a thread rather than one, so that fewer waves wait for each other: 8192
+        // x 8192 bf16 97 us against 108, 4096 x 4096 fp16 12.2 against 14.7, 8 x 8192 3.9 and
+        // 3.9; but one where that makes 512 threads and the rows leave CUs free: 1 x 4096 2.1
+        // against 2.3.
+        const int cus = num_cus();
+        if (n <= 64) return launch<T, 64, 1>(a, cus, s);
+        if (n <= 128) return launch<T, 64, 2>(a, cus, s);
+        if (n <= 256) return launch<T, 256, 1>(a, cus, s);
+        if (n <= 512) return a.rows <= cus ? launch<T, 512, 1>(a, cus, s) : launch<T, 256, 2>(a, cus, s);
+        if (n <= 1024) return launch<T, 512, 2>(a, cus, s);
+        if (n <= 2048) return launch<T, 1024, 2>(a, cus, s);
+        if (n <= 4096) return launch<T, 1024, 4>(a, cus, s);
+        if constexpr (VN == 4) return launch<T, 1024, 8>(a, cus, s);
         return false;
     });
 }
