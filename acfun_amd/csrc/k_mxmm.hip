@@ -119,7 +119,11 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
         i4v a[U][TM], b[U][TN];
         unsigned sa[TM], sb[TN];
     };
-    auto load = [&](Unit& r, unsigned u) {
+    // A wave's units: 2^run neighbours at a time, which one load of scales serves, as long as
+    // every wave has that many.
+    const int run = U == 4 ? 0 : units >= 4 / U * W ? (U == 1 ? 2 : 1) : U == 1 && units >= 2 * W ? 1 : 0;
+    auto unit = [&](unsigned i) { return (((i >> run) * W + w) << run) + (i & ((1 << run) - 1)); };
+    auto load = [&](Unit& r, unsigned u, bool scales) {
         const uint64_t g = (uint64_t)(u * U >> 2) << 8;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -130,6 +134,7 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
 #pragma unroll
                 for (int j = 0; j < TM; ++j) r.a[i][j] = *(const i4v*)(a[j] + k + o16);
         }
+        if (U < 4 && !scales) return;
 #pragma unroll
         for (int j = 0; j < TN; ++j) r.sb[j] = *(const unsigned*)(bs[j] + g + o4);
         if constexpr (!ROWS)
@@ -193,16 +198,18 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
         }
     };
     Unit r;
-    if (w < units) load(r, w);
+    unsigned u = unit(0);
+    if (u < units) load(r, u, true);
     if constexpr (ROWS) {
         if (p.K % 512 == 0) quantize(std::integral_constant<int, 0>{});
         else if (p.K % 8 == 0) quantize(std::integral_constant<int, 1>{});
         else quantize(std::integral_constant<int, 2>{});
         __syncthreads();
     }
-    for (unsigned u = w; u < units; u += W) {
+    for (unsigned i = 0; u < units;) {
         Unit c = r;
-        if (u + W < units) load(r, u + W);
+        const unsigned v = unit(++i);
+        if (v < units) load(r, v, (i & ((1 << run) - 1)) == 0);
         take_rows(c, u);
         if constexpr (U < 4) {
             const int sh = 8 * ((u * U) & 3);
@@ -212,7 +219,7 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
             for (int j = 0; j < TM; ++j) c.sa[j] >>= sh;
         }
         each<U>([&](auto ic) {
-            constexpr int i = decltype(ic)::value;
+            constexpr int i = decltype(ic)::value;          // of the unit's U
             if (i > 0 && u * U + i >= kt) return;
 #pragma unroll
             for (int y = 0; y < TM; ++y)
@@ -221,6 +228,7 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
                     acc[y][x] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
                         wide(c.b[i][x]), wide(c.a[i][y]), acc[y][x], 4, 4, i, c.sb[x], i, c.sa[y]);
         });
+        u = v;
     }
 #pragma unroll
     for (int y = 0; y < TM; ++y)
@@ -522,9 +530,9 @@ bool launch_many(MmArgs a, hipStream_t s) {
 // 546 sizes (M of 16 to 8192, N of 64 to 8192, K of 128 to 8192; bf16, replayed from a
 // graph): a call takes `lat` while the CUs have less than a tile each, and `base` and
 // `each` times the tiles of a CU from there.  The tile chosen is 0.8 % slower than the
-// best of each size in the mean.  Measured, us: 128 x 8192 x 4096 9.7 with tiles of 32,
-// 6.8 with 64, 11.3 with 128; 512 x 8192 x 1024 15 with 64, 7.1 with 128; 2048 x 8192 x
-// 4096 45 with 128, 38 with 256.
+// best of each size in the mean.  Measured, us: 128 x 8192 x 4096 9.4 with tiles of 32,
+// 8.0 with 64, 11.0 with 128; 512 x 8192 x 1024 14.2 with 64, 6.7 with 128; 8192 x 8192 x
+// 4096 154 with 128, 136 with 256 (other operands each time).
 double tile_time(double lat, double base, double each, double tiles_per_cu) {
     const double t = base + each * tiles_per_cu;
     return t > lat ? t : lat;
@@ -540,11 +548,11 @@ MmKind mm_choose(int M, int N, int K, double cus, double& us) {
     };
     auto more = [](double a, double b) { return a > b ? a : b; };
     const double t[KINDS] = {
-        tile_time(2.72 + 0.91e-4 * k, 2.05 + 1.1e-4 * k, 0.417 + 1.55e-4 * k, per_cu(16)),
-        tile_time(0.8 + 5.5e-4 * k, 2.76 + 2.8e-4 * k, more(0.235 + 2.0e-4 * k, 4.0e-4 * k), per_cu(32)),
-        tile_time(3.81 + 7.9e-4 * k, 2.05 + 2.9e-4 * k, 2.41 + 8.7e-4 * k, per_cu(64)),
-        tile_time(3.89 + 17.2e-4 * k, 3.79 + 4.4e-4 * k, 1.51 + 19.8e-4 * k, per_cu(128)),
-        tile_time(7.36 + 43.7e-4 * k, 3.73, more(8.04 + 67.6e-4 * k, 77.4e-4 * k), per_cu(256)),
+        tile_time(2.72 + 0.89e-4 * k, 2.18 + 0.64e-4 * k, more(0.42 + 1.12e-4 * k, 2.42e-4 * k), per_cu(16)),
+        tile_time(2.73, 2.73 + 2.7e-4 * k, more(0.247 + 1.74e-4 * k, 3.8e-4 * k), per_cu(32)),
+        tile_time(3.57 + 6.6e-4 * k, 1.91 + 2.65e-4 * k, 2.3 + 8.2e-4 * k, per_cu(64)),
+        tile_time(3.87 + 17.6e-4 * k, 3.88 + 2.9e-4 * k, 1.39 + 18.8e-4 * k, per_cu(128)),
+        tile_time(7.28 + 43.5e-4 * k, 4.37 + 1.6e-4 * k, 7.32 + 63.7e-4 * k, per_cu(256)),
     };
     // 32-bit offsets into a tile's operands
     const int kinds = K > 0 && K <= (1 << 22) ? KINDS : MANY128;
