@@ -3,8 +3,10 @@
 // Memory bounds them: max|x| of a block is found among the threads that hold it, so
 // a value is read once.  Measured: 4096 x 4096 bf16 7.9 us and back 7.4 (42 MB each, 5.5
 // TB/s), fp32 weights [4096][8192] 25.6 (152 MB, 5.9 TB/s; operands that the caches held
-// from the call before); with a thread to a block and its 32 values read one by one
-// 166 for both and 749 there and back.
+// from the call before), there and back with others each time 56; with a thread to a
+// block and its 32 values read one by one 166 and 749 there and back.
+#include <type_traits>
+
 #include "mx.hpp"
 
 namespace acfun {
@@ -79,40 +81,59 @@ __global__ __launch_bounds__(256) void k_mx_quant_t(const T* __restrict__ x, int
             bytes[0][l] | bytes[1][l] << 8 | bytes[2][l] << 16 | bytes[3][l] << 24;
 }
 
-// The threads of k_mx_quant, the other way.
+// The other way.  A thread has V values (16 bytes) of each part of a row's 128 k, so
+// that 16 threads store 256 consecutive bytes: eight bf16 or fp16 of one part, four fp32
+// of each of two, for which the codes are read as halves of dwords.  Rows of whole
+// cache lines are stored past the caches; of others the caches join the parts.
 template <class T>
 __global__ __launch_bounds__(256) void k_mx_dequant(const uint8_t* __restrict__ codes,
                                                     const uint8_t* __restrict__ scales, int rows, int K, int st,
                                                     T* __restrict__ x) {
-    const int t = threadIdx.x, r = t >> 4, j = (t >> 2) & 3, p = t & 3;
+    constexpr int V = 16 / (int)sizeof(T), H = 8 / V;
+    const int t = threadIdx.x, r = t >> 4, l = t & 15;
     const int rt = (int)(blockIdx.x / (unsigned)st), b = (int)(blockIdx.x - (unsigned)rt * st);
     const int kt = mx_k_tiles(K), left = K - 512 * b;
     const unsigned row = rt * 16u + r;
     if (row >= (unsigned)rows) return;
-    const size_t lane = 16 * j + r;
-    const unsigned bytes = ((const unsigned*)scales)[((size_t)rt * st + b) * 64 + lane];
-    unsigned c[4];
+    unsigned bytes[H], c[4][H];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-        c[s] = 4 * b + s < kt ? ((const unsigned*)codes)[(((size_t)rt * kt + 4 * b + s) * 64 + lane) * 4 + p] : 0;
-    T* xr = x + (size_t)row * K + 512 * b;
+    for (int h = 0; h < H; ++h) {
+        const int k = 16 * V * h + V * l;                       // of the 128
+        const size_t lane = 16 * (k >> 5) + r;
+        bytes[h] = ((const unsigned*)scales)[((size_t)rt * st + b) * 64 + lane];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const int k = 128 * s + 32 * j + 8 * p;
-        const unsigned byte = (bytes >> (8 * s)) & 255u;
-        const float scale = mx_scale_float(byte == 255 ? 0 : byte);
-        float f[8];
-        auto pair = [&](int e, auto v) {
-            f[e] = byte == 255 ? __uint_as_float(0x7fc00000u) : v[0];
-            f[e + 1] = byte == 255 ? __uint_as_float(0x7fc00000u) : v[1];
-        };
-        pair(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s], scale, 0));
-        pair(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s], scale, 1));
-        pair(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s], scale, 2));
-        pair(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s], scale, 3));
-        // (a lane's eight fp32 values are two stores of half lines, which the caches join)
-        if (k < left) store_vec<T, 8, sizeof(T) == 2>(xr + k, left - k, f);
+        for (int s = 0; s < 4; ++s)
+            c[s][h] = 4 * b + s < kt ? ((const unsigned*)codes)[(((size_t)rt * kt + 4 * b + s) * 64 + lane) * 4 +
+                                                                (k >> 3 & 3)] >> 4 * (k & 7) : 0;
     }
+    T* xr = x + (size_t)row * K + 512 * b;
+    // ENDS: 0 rows of whole cache lines, 1 of whole 16 bytes, 2 others
+    auto put = [&](auto ENDS) {
+        constexpr int ends = decltype(ENDS)::value;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const int k = 128 * s + 16 * V * h + V * l;
+                const unsigned byte = (bytes[h] >> (8 * s)) & 255u;
+                const float scale = mx_scale_float(byte == 255 ? 0 : byte);
+                float f[V];
+                auto pair = [&](int e, auto v) {
+                    f[e] = byte == 255 ? __uint_as_float(0x7fc00000u) : v[0];
+                    f[e + 1] = byte == 255 ? __uint_as_float(0x7fc00000u) : v[1];
+                };
+                pair(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s][h], scale, 0));
+                pair(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s][h], scale, 1));
+                if constexpr (V == 8) {
+                    pair(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s][h], scale, 2));
+                    pair(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[s][h], scale, 3));
+                }
+                if (k < left) store_vec<T, V, ends == 0>(xr + k, ends < 2 ? V : left - k, f);
+            }
+    };
+    if (K % (8 * V) == 0) put(std::integral_constant<int, 0>{});
+    else if (K % V == 0) put(std::integral_constant<int, 1>{});
+    else put(std::integral_constant<int, 2>{});
 }
 
 bool grid_ok(long long n, const char* what) {

@@ -6,7 +6,7 @@
 // k_mxmm_few: tiles of 16, 32 or 64 on the 16 x 16 x 128 MFMA, K split between a
 // workgroup's waves.  A launch's latency bounds the smallest, the reading of the weights
 // the others: 1 x 4096 x 4096 3.5 us in a graph with the quantization of its row, 1 x
-// 16384 -> 4096 8.4 (34 MB, 4 TB/s), 128 x 8192 x 4096 6.8.
+// 16384 -> 4096 8.4 (34 MB, 4 TB/s), 128 x 8192 x 4096 6.7.
 //
 // k_mxmm: four waves of 2 x 2 or 4 x 4 blocks of 32 x 32, operands DMA'd into LDS in
 // chunks of 128 k, four stages.  The 256 x 256 tile needs 512 bytes of LDS reads per
