@@ -39,6 +39,7 @@ struct Checks {
         return out == in ? *this : apart(out, n, in, n);
     }
     Checks& param(const float* p) { return need((uintptr_t)p % 4 == 0, "a parameter is not aligned to 4 bytes"); }
+    Checks& fits(bool f) { return need(f, "too large: a launch holds fewer than 2^32 threads"); }
     Checks& held(const uint8_t* codes, const uint8_t* scales) {
         need(codes && scales, "codes or scales are NULL");
         return need((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0,
@@ -90,7 +91,7 @@ int acfun_dev_quantize_mxfp4(const void* x, int type, int rows, int K, int trans
     const size_t n = (size_t)rows * K * type_size(type);
     c.apart(codes, mx_code_bytes(rows, K), x, n).apart(scales, mx_scale_bytes(rows, K), x, n);
     c.apart(codes, mx_code_bytes(rows, K), scales, mx_scale_bytes(rows, K));
-    if (!c.ok) return -1;
+    if (!c.fits(mx_quant_fits(rows, K, trans)).ok) return -1;
     return call(c.who, [&] { return mx_quantize(x, type, rows, K, trans, codes, scales, resolve(stream)); });
 }
 
@@ -102,6 +103,7 @@ int acfun_dev_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, int 
     if (!c.tensor(x, type, "x is NULL").held(codes, scales).ok) return -1;
     const size_t n = (size_t)rows * K * type_size(type);
     if (!c.apart(x, n, codes, mx_code_bytes(rows, K)).apart(x, n, scales, mx_scale_bytes(rows, K)).ok) return -1;
+    if (!c.fits(mx_quant_fits(rows, K, 0)).ok) return -1;
     return call(c.who, [&] { return mx_dequantize(codes, scales, rows, K, x, type, resolve(stream)); });
 }
 
@@ -117,7 +119,7 @@ int acfun_dev_gemm_mxfp4(int M, int N, int K, const uint8_t* A, const uint8_t* a
         c.apart(C, n, A, mx_code_bytes(M, K)).apart(C, n, a_scales, mx_scale_bytes(M, K));
         c.apart(C, n, B, mx_code_bytes(N, K)).apart(C, n, b_scales, mx_scale_bytes(N, K));
     }
-    if (!c.apart(C, n, bias, 4 * (size_t)N).ok) return -1;
+    if (!c.apart(C, n, bias, 4 * (size_t)N).fits(mm_fits(M, N, K)).ok) return -1;
     return call(c.who, [&] {
         return mx_gemm(M, N, K, A, a_scales, B, b_scales, C, type, bias, act, resolve(stream));
     });
@@ -135,7 +137,7 @@ int acfun_dev_fc_mxfp4(const void* input, int type, int N, int Cin, const uint8_
         c.apart(output, n, input, (size_t)N * Cin * type_size(type));
         c.apart(output, n, weight, mx_code_bytes(Cout, Cin)).apart(output, n, wscale, mx_scale_bytes(Cout, Cin));
     }
-    if (!c.apart(output, n, bias, 4 * (size_t)Cout).ok) return -1;
+    if (!c.apart(output, n, bias, 4 * (size_t)Cout).fits(fc_fits(N, Cout, Cin)).ok) return -1;
     return call(c.who, [&] {
         return mx_fc(input, type, N, Cin, weight, wscale, bias, Cout, output, act, resolve(stream));
     });

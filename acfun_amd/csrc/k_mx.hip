@@ -18,7 +18,7 @@ namespace {
 // threads read 128 consecutive k of a row, four of them share a block, and a wave
 // writes 64 consecutive bytes of codes to each of four places.
 template <class T>
-__global__ __launch_bounds__(256) void k_mx_quant(const T* __restrict__ x, int rows, int K, int st,
+__global__ __launch_bounds__(kMxThreads) void k_mx_quant(const T* __restrict__ x, int rows, int K, int st,
                                                   uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     const int t = threadIdx.x, r = t >> 4, j = (t >> 2) & 3, p = t & 3;
     const int rt = (int)(blockIdx.x / (unsigned)st), b = (int)(blockIdx.x - (unsigned)rt * st);
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void k_mx_quant(const T* __restrict__ x, int r
 // of a scale tile; wave s has the s-th 128 k and lane r a row, so that a wave reads
 // 64 neighbours of each k and writes 256 consecutive bytes of codes.
 template <class T>
-__global__ __launch_bounds__(256) void k_mx_quant_t(const T* __restrict__ x, int rows, int K, int groups,
+__global__ __launch_bounds__(kMxThreads) void k_mx_quant_t(const T* __restrict__ x, int rows, int K, int groups,
                                                     int st, uint8_t* __restrict__ codes,
                                                     uint8_t* __restrict__ scales) {
     __shared__ unsigned bytes[4][64];
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void k_mx_quant_t(const T* __restrict__ x, int
 // of each of two, for which the codes are read as halves of dwords.  Rows of whole
 // cache lines are stored past the caches; of others the caches join the parts.
 template <class T>
-__global__ __launch_bounds__(256) void k_mx_dequant(const uint8_t* __restrict__ codes,
+__global__ __launch_bounds__(kMxThreads) void k_mx_dequant(const uint8_t* __restrict__ codes,
                                                     const uint8_t* __restrict__ scales, int rows, int K, int st,
                                                     T* __restrict__ x) {
     constexpr int V = 16 / (int)sizeof(T), H = 8 / V;
@@ -136,27 +136,20 @@ __global__ __launch_bounds__(256) void k_mx_dequant(const uint8_t* __restrict__ 
     else put(std::integral_constant<int, 2>{});
 }
 
-bool grid_ok(long long n, const char* what) {
-    if (n < (1ll << 31)) return true;
-    set_error("%s: too large", what);
-    return false;
-}
-
 }  // namespace
 
 bool mx_quantize(const void* x, int type, int rows, int K, int trans, uint8_t* codes, uint8_t* scales,
                  hipStream_t s) {
     const long long st = mx_scale_tiles(K), groups = ((long long)rows + 63) / 64;
-    const long long grid = trans ? groups * st * 4 : mx_row_tiles(rows) * st;
-    if (!grid_ok(grid, "acfun_dev_quantize_mxfp4")) return false;
+    const long long grid = mx_quant_groups(rows, K, trans);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         if (trans) {
-            ACFUN_LAUNCH("k_mx_quant_t", (k_mx_quant_t<T>), dim3((unsigned)grid), dim3(256), 0, s, (const T*)x,
+            ACFUN_LAUNCH("k_mx_quant_t", (k_mx_quant_t<T>), dim3((unsigned)grid), dim3(kMxThreads), 0, s, (const T*)x,
                          rows, K, (int)groups, (int)st, codes, scales);
             return check_launch("k_mx_quant_t");
         }
-        ACFUN_LAUNCH("k_mx_quant", (k_mx_quant<T>), dim3((unsigned)grid), dim3(256), 0, s, (const T*)x, rows, K,
+        ACFUN_LAUNCH("k_mx_quant", (k_mx_quant<T>), dim3((unsigned)grid), dim3(kMxThreads), 0, s, (const T*)x, rows, K,
                      (int)st, codes, scales);
         return check_launch("k_mx_quant");
     });
@@ -164,11 +157,10 @@ bool mx_quantize(const void* x, int type, int rows, int K, int trans, uint8_t* c
 
 bool mx_dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int K, void* x, int type,
                    hipStream_t s) {
-    const long long st = mx_scale_tiles(K), grid = mx_row_tiles(rows) * st;
-    if (!grid_ok(grid, "acfun_dev_dequantize_mxfp4")) return false;
+    const long long st = mx_scale_tiles(K), grid = mx_quant_groups(rows, K, 0);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        ACFUN_LAUNCH("k_mx_dequant", (k_mx_dequant<T>), dim3((unsigned)grid), dim3(256), 0, s, codes, scales, rows,
+        ACFUN_LAUNCH("k_mx_dequant", (k_mx_dequant<T>), dim3((unsigned)grid), dim3(kMxThreads), 0, s, codes, scales, rows,
                      K, (int)st, (T*)x);
         return check_launch("k_mx_dequant");
     });

@@ -70,12 +70,6 @@ struct MmArgs {
 // memory to registers, and so does A if X is void.  Otherwise A is float rows of X,
 // which the workgroup quantizes into LDS for its tile, while B's first loads are on
 // their way.
-template <int TM, int TN, int W>
-constexpr size_t kFewSums = (size_t)W * TM * TN * 68 * 16;
-// The LDS of quantized rows: room for 1, 2, 4, 8 or 16 of them.
-inline int few_rows(int M) { return M > 8 ? 16 : M > 4 ? 8 : M > 2 ? 4 : M; }
-inline size_t few_rows_lds(int M, int K) { return (size_t)few_rows(M) * mx_scale_tiles(K) * (256 + 16); }
-
 template <class T, class X, int TM, int TN, int W, int U>
 __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
     constexpr bool ROWS = !std::is_void_v<X>;
@@ -488,18 +482,14 @@ bool launch_few(MmArgs a, hipStream_t s) {
     // set once per process, thread-safely, before any launch below
     static const bool attr = [] {
         (void)hipFuncSetAttribute((const void*)k_mxmm_few<T, X, TM, TN, W, U>,
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
         return true;
     }();
     (void)attr;
     a.gm = (int)((mx_row_tiles(a.M) + TM - 1) / TM);
     a.gn = (int)((mx_row_tiles(a.N) + TN - 1) / TN);
     a.rows = few_rows(a.M);
-    const long long grid = ((long long)a.gm * a.gn + 7) / 8 * 8;
-    if (grid >= (1ll << 31)) {
-        set_error("acfun_dev_gemm_mxfp4: too large");
-        return false;
-    }
+    const long long grid = xcd_groups((long long)a.gm * a.gn);
     ACFUN_LAUNCH("k_mxmm_few", (k_mxmm_few<T, X, TM, TN, W, U>), dim3((unsigned)grid), dim3(64 * W),
                  (kFewSums<TM, TN, W> + (std::is_void_v<X> ? 0 : few_rows_lds(a.M, a.K))), s, a);
     return check_launch("k_mxmm_few");
@@ -508,7 +498,7 @@ bool launch_few(MmArgs a, hipStream_t s) {
 template <class T, int FM, int FN>
 bool launch_many(MmArgs a, hipStream_t s) {
     using Tl = MmTile<FM, FN>;
-    static_assert(Tl::LDS <= 160 * 1024, "LDS");
+    static_assert(Tl::LDS <= kLds, "LDS");
     // set once per process, thread-safely, before any launch below
     static const bool attr = [] {
         (void)hipFuncSetAttribute((const void*)k_mxmm<T, FM, FN>, hipFuncAttributeMaxDynamicSharedMemorySize, Tl::LDS);
@@ -517,61 +507,9 @@ bool launch_many(MmArgs a, hipStream_t s) {
     (void)attr;
     a.gm = (int)(((long long)a.M + Tl::BM - 1) / Tl::BM);
     a.gn = (int)(((long long)a.N + Tl::BN - 1) / Tl::BN);
-    const long long grid = ((long long)a.gm * a.gn + 7) / 8 * 8;
-    if (grid >= (1ll << 31)) {
-        set_error("acfun_dev_gemm_mxfp4: too large");
-        return false;
-    }
+    const long long grid = xcd_groups((long long)a.gm * a.gn);
     ACFUN_LAUNCH("k_mxmm", (k_mxmm<T, FM, FN>), dim3((unsigned)grid), dim3(256), Tl::LDS, s, a);
     return check_launch("k_mxmm");
-}
-
-// Times in us that choose a kernel and its tile, fitted to those of every tile over
-// 546 sizes (M of 16 to 8192, N of 64 to 8192, K of 128 to 8192; bf16, replayed from a
-// graph): a call takes `lat` while the CUs have less than a tile each, and `base` and
-// `each` times the tiles of a CU from there.  The tile chosen is 0.8 % slower than the
-// best of each size in the mean.  Measured, us: 128 x 8192 x 4096 9.4 with tiles of 32,
-// 8.0 with 64, 11.0 with 128; 512 x 8192 x 1024 14.2 with 64, 6.7 with 128; 8192 x 8192 x
-// 4096 154 with 128, 136 with 256 (other operands each time).
-double tile_time(double lat, double base, double each, double tiles_per_cu) {
-    const double t = base + each * tiles_per_cu;
-    return t > lat ? t : lat;
-}
-
-enum MmKind { FEW16, FEW32, FEW64, MANY128, MANY256, KINDS };
-
-// The fastest kernel for a product, and its time.
-MmKind mm_choose(int M, int N, int K, double cus, double& us) {
-    const double k = K;
-    auto per_cu = [&](int b) {
-        return (double)(((long long)M + b - 1) / b) * (double)(((long long)N + b - 1) / b) / cus;
-    };
-    auto more = [](double a, double b) { return a > b ? a : b; };
-    const double t[KINDS] = {
-        tile_time(2.72 + 0.89e-4 * k, 2.18 + 0.64e-4 * k, more(0.42 + 1.12e-4 * k, 2.42e-4 * k), per_cu(16)),
-        tile_time(2.73, 2.73 + 2.7e-4 * k, more(0.247 + 1.74e-4 * k, 3.8e-4 * k), per_cu(32)),
-        tile_time(3.57 + 6.6e-4 * k, 1.91 + 2.65e-4 * k, 2.3 + 8.2e-4 * k, per_cu(64)),
-        tile_time(3.87 + 17.6e-4 * k, 3.88 + 2.9e-4 * k, 1.39 + 18.8e-4 * k, per_cu(128)),
-        tile_time(7.28 + 43.5e-4 * k, 4.37 + 1.6e-4 * k, 7.32 + 63.7e-4 * k, per_cu(256)),
-    };
-    // 32-bit offsets into a tile's operands
-    const int kinds = K > 0 && K <= (1 << 22) ? KINDS : MANY128;
-    int best = 0;
-    for (int i = 1; i < kinds; ++i)
-        if (t[i] < t[best]) best = i;
-    us = t[best];
-    return (MmKind)best;
-}
-
-// The same for a layer whose workgroups each quantize their 16 rows, with tiles of 16,
-// 32 or 64 columns (tn tiles of 16): `pieces` of a row and 512 k fall to each wave.
-// Where LDS has no room for the rows it cannot be done.
-double rows_time(int M, int N, int K, double cus, int tn) {
-    if (kFewSums<1, 1, 8> * tn + few_rows_lds(M, K) > 160 * 1024) return 1e30;
-    const double k = K, pieces = (double)(((M < 16 ? M : 16) * (long long)mx_scale_tiles(K) + 7) / 8);
-    const double per_cu = (double)mx_row_tiles(M) * (double)((mx_row_tiles(N) + tn - 1) / tn) / cus;
-    return tile_time(3.05 + 0.037 * tn + (0.94e-4 * tn - 0.77e-4) * k + 0.167 * pieces, 2.4 + 0.13 * pieces,
-                     0.42 + 0.132 * tn + (1.32e-4 + 0.78e-4 * tn) * k + 0.074 * pieces, per_cu);
 }
 
 }  // namespace
@@ -595,23 +533,12 @@ bool mx_gemm(int M, int N, int K, const uint8_t* A, const uint8_t* As, const uin
 bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_t* Bs, const float* bias,
            int N, void* C, int act, hipStream_t s) {
     if (K > 0) {
-        // One launch, in which every workgroup quantizes its 16 rows, or two, of which the
-        // first takes 2.45 us and its traffic at 4.5 TB/s?  Measured, us: 16 x 2048 x 2048 4.4
-        // and 5.0, 16 x 2048 x 8192 9.0 and 6.1; 128 x 2048 x 1024 4.3 and 5.7, 333 x 2048 x
-        // 2048 10.1 and 8.2.
-        const double cus = num_cus();
-        double two, one = rows_time(M, N, K, cus, 1);
-        (void)mm_choose(M, N, K, cus, two);
-        two += 2.45 + (double)M * K * (type_size(type) + 0.53) * 0.22e-6;
-        int tn = 1;
-        for (int n = 2; n <= 4; n *= 2)
-            if (const double t = rows_time(M, N, K, cus, n); t < one) one = t, tn = n;
-        if (one < two) {
+        if (const FcPlan plan = fc_plan(M, N, K, type_size(type), num_cus()); plan.one) {
             const MmArgs a{M, N, K, x, nullptr, B, Bs, C, bias, act, 0, 0};
             return with_type(type, [&](auto t) {
                 using T = decltype(t);
-                if (tn == 1) return launch_few<T, T, 1, 1, 8, 4>(a, s);
-                if (tn == 2) return launch_few<T, T, 1, 2, 8, 4>(a, s);
+                if (plan.tn == 1) return launch_few<T, T, 1, 1, 8, 4>(a, s);
+                if (plan.tn == 2) return launch_few<T, T, 1, 2, 8, 4>(a, s);
                 return launch_few<T, T, 1, 4, 8, 2>(a, s);
             });
         }

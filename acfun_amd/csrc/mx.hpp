@@ -18,6 +18,7 @@
 // Rows are padded to 16, codes to 128 k and scales to 512 k; the quantizer
 // writes zeros there.
 #pragma once
+#include "mx_plan.hpp"
 #include "rt.hpp"
 
 namespace acfun {
@@ -78,12 +79,6 @@ __device__ __forceinline__ unsigned lane_perm(unsigned v) {
     return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;
-
-__host__ __device__ inline long long mx_row_tiles(int rows) { return ((long long)rows + 15) / 16; }
-__host__ __device__ inline int mx_k_tiles(int K) { return (int)(((long long)K + 127) / 128); }
-__host__ __device__ inline int mx_scale_tiles(int K) { return (int)(((long long)K + 511) / 512); }
-inline size_t mx_code_bytes(int rows, int K) { return (size_t)mx_row_tiles(rows) * mx_k_tiles(K) * 1024; }
-inline size_t mx_scale_bytes(int rows, int K) { return (size_t)mx_row_tiles(rows) * mx_scale_tiles(K) * 256; }
 
 // Eight values -> eight codes.
 __device__ __forceinline__ unsigned mx_codes8(const float* v, float scale) {

@@ -253,7 +253,8 @@ int acfun_dev_softmax(const float* input, int rows, int cols, float* output, voi
  * The acfun_dev_* calls take device pointers and a stream as above; they return
  * 0, or -1 with acfun_last_error() and nothing queued: on a negative size, an
  * unknown type or code, a NULL or misaligned pointer, a result that overlaps an
- * input (but where a call says that it may be one).  An empty output is 0. */
+ * input (but where a call says that it may be one), sizes beyond a launch (some 2^32
+ * threads: 2^28 rows of up to 512 to 4 bits).  An empty output is 0. */
 #define ACFUN_F32 0
 #define ACFUN_BF16 1
 #define ACFUN_F16 2
