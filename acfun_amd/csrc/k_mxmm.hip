@@ -533,7 +533,20 @@ bool mx_gemm(int M, int N, int K, const uint8_t* A, const uint8_t* As, const uin
 bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_t* Bs, const float* bias,
            int N, void* C, int act, hipStream_t s) {
     if (K > 0) {
-        if (const FcPlan plan = fc_plan(M, N, K, type_size(type), num_cus()); plan.one) {
+        const FcPlan plan = fc_plan(M, N, K, type_size(type), num_cus());
+        bool one = plan.one;
+        if (!one) {
+            // a graph would keep the addresses of temporaries that go back to the pool here
+            hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
+            if (!check(hipStreamIsCapturing(s, &captured), "hipStreamIsCapturing")) return false;
+            one = captured != hipStreamCaptureStatusNone;
+            if (one && !plan.captured) {
+                set_error("acfun_dev_fc_mxfp4: these sizes need temporaries, which a graph cannot keep: capture "
+                          "acfun_dev_quantize_mxfp4 and acfun_dev_gemm_mxfp4 with buffers of the caller's");
+                return false;
+            }
+        }
+        if (one) {
             const MmArgs a{M, N, K, x, nullptr, B, Bs, C, bias, act, 0, 0};
             return with_type(type, [&](auto t) {
                 using T = decltype(t);
@@ -542,14 +555,6 @@ bool mx_fc(const void* x, int type, int M, int K, const uint8_t* B, const uint8_
                 return launch_few<T, T, 1, 4, 8, 2>(a, s);
             });
         }
-    }
-    // a graph would keep the addresses of temporaries that go back to the pool here
-    hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
-    if (K > 0 && !check(hipStreamIsCapturing(s, &captured), "hipStreamIsCapturing")) return false;
-    if (captured != hipStreamCaptureStatusNone) {
-        set_error("acfun_dev_fc_mxfp4: these sizes need temporaries, which a graph cannot keep: capture "
-                  "acfun_dev_quantize_mxfp4 and acfun_dev_gemm_mxfp4 with buffers of the caller's");
-        return false;
     }
     Scratch codes(mx_code_bytes(M, K), s), scales(mx_scale_bytes(M, K), s);
     if (K > 0 && (!codes.p || !scales.p)) return false;

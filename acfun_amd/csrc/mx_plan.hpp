@@ -110,9 +110,15 @@ constexpr bool fc_fits(int M, int N, int K) {
            (K > 0 && (rows_fits(M, N, K, 1) || rows_fits(M, N, K, 2) || rows_fits(M, N, K, 4)));
 }
 
+// The rows up to which a layer is always one launch while its stream is captured into a
+// graph, where LDS has room for 16 of them: two launches need a temporary, which a graph
+// cannot keep, and programs that capture have to know beforehand what they may.
+constexpr int kCapturedRows = 512;
+
 struct FcPlan {
-    int tn;                         // tiles of a workgroup that quantizes its rows
-    bool one;                       // one launch of those, or two
+    int tn;                         // tiles of a workgroup that quantizes its rows; 0: LDS has no room for them
+    bool one;                       // one launch of those is faster than two
+    bool captured;                  // one launch is taken on a captured stream
 };
 // One launch, in which every workgroup quantizes its 16 rows, or two, of which the
 // first takes 2.45 us and its traffic at 4.5 TB/s?  Measured, us: 16 x 2048 x 2048 4.4
@@ -122,10 +128,10 @@ inline FcPlan fc_plan(int M, int N, int K, size_t elem, double cus) {
     double two, one = kNever;
     (void)mm_choose(M, N, K, cus, two);
     two = mx_quant_fits(M, K, 0) ? two + 2.45 + (double)M * K * (elem + 0.53) * 0.22e-6 : kNever;
-    int tn = 1;
+    int tn = 0;
     for (int n = 1; n <= 4; n *= 2)
         if (const double t = rows_time(M, N, K, cus, n); t < one) one = t, tn = n;
-    return {tn, one < two};
+    return {tn, one < two, one < two || (tn && M <= kCapturedRows)};
 }
 
 }  // namespace acfun

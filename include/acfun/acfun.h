@@ -290,10 +290,13 @@ int acfun_dev_gemm_mxfp4(int M, int N, int K, const uint8_t* A, const uint8_t* a
                          const float* bias, int act, void* stream);
 /* A fully connected layer with weights held in MXFP4 (an operand of Cout rows):
  * input [N, Cin] is quantized as acfun_dev_quantize_mxfp4 does and multiplied;
- * output [N, Cout].  Input and output are of `type`.  Small layers are one launch
- * without temporaries; for others the quantized input lies in the library's pool, and
- * a call on a stream that is being captured into a graph is refused: quantize into
- * buffers of the caller's and multiply, which is the same.  */
+ * output [N, Cout].  Input and output are of `type`.  The call is one launch without
+ * temporaries, or two with the quantized input in the library's pool, whichever is the
+ * faster.  On a stream that is being captured into a graph it is one launch for any N of
+ * at most 512, Cin of at most 17920 (36352 for N of at most 8) and Cout of at most four
+ * million; past that it may be refused, and quantizing into buffers of the caller's and
+ * multiplying is the same.  The forms add in different orders, so their results may
+ * differ by their sums' rounding. */
 int acfun_dev_fc_mxfp4(const void* input, int type, int N, int Cin, const uint8_t* weight,
                        const uint8_t* wscale, const float* bias, int Cout, void* output, int act,
                        void* stream);

@@ -1,6 +1,7 @@
 // Prints the plan (acfun_amd/csrc/mx_plan.hpp) of each line of the input:
 //   gemm M N K cus          -> the kind, or none
-//   fc M N K elem cus       -> rows16 | rows32 | rows64 (one launch) or two
+//   fc M N K elem cus       -> rows16 | rows32 | rows64 (one launch), two, or two/rows.. (two, but the
+//                              one on a captured stream)
 //   quant rows K trans      -> fits or not
 #include <cstdio>
 #include <cstring>
@@ -24,6 +25,7 @@ int main() {
             if (std::scanf("%d %d", &elem, &cus) != 2) return 1;
             const FcPlan p = fc_plan(a, b, c, (size_t)elem, cus);
             if (p.one) std::printf("rows%d\n", 16 * p.tn);
+            else if (p.captured) std::printf("two/rows%d\n", 16 * p.tn);
             else std::puts("two");
         } else {
             std::puts(mx_quant_fits(a, b, c) ? "fits" : "not");
