@@ -112,7 +112,10 @@ constexpr bool fc_fits(int M, int N, int K) {
 
 // The rows up to which a layer is always one launch while its stream is captured into a
 // graph, where LDS has room for 16 of them: two launches need a temporary, which a graph
-// cannot keep, and programs that capture have to know beforehand what they may.
+// cannot keep, and programs that capture have to know beforehand what they may.  Measured
+// in a graph, us, against two calls on the caller's buffers: 16 x 4096 x 4096 6.4 and 5.6,
+// 128 x 4096 x 4096 10.7 and 9.4, 512 x 4096 x 4096 35.6 and 15.4, 512 x 8192 x 8192 196
+// and 26.
 constexpr int kCapturedRows = 512;
 
 struct FcPlan {

@@ -294,9 +294,10 @@ int acfun_dev_gemm_mxfp4(int M, int N, int K, const uint8_t* A, const uint8_t* a
  * temporaries, or two with the quantized input in the library's pool, whichever is the
  * faster.  On a stream that is being captured into a graph it is one launch for any N of
  * at most 512, Cin of at most 17920 (36352 for N of at most 8) and Cout of at most four
- * million; past that it may be refused, and quantizing into buffers of the caller's and
- * multiplying is the same.  The forms add in different orders, so their results may
- * differ by their sums' rounding. */
+ * million; past that it may be refused.  Quantizing into buffers of the caller's and
+ * multiplying is the same, can be captured at any size, and from some 128 rows on takes
+ * less time in a graph than the one launch does.  The forms add in different orders, so
+ * their results may differ by their sums' rounding. */
 int acfun_dev_fc_mxfp4(const void* input, int type, int N, int Cin, const uint8_t* weight,
                        const uint8_t* wscale, const float* bias, int Cout, void* output, int act,
                        void* stream);
