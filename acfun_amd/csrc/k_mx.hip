@@ -1,8 +1,8 @@
 // k_mx.hip -- the MXFP4 quantizer and its inverse (layout and rounding: mx.hpp).
 //
 // Memory bounds them: max|x| of a block is found among the threads that hold it, so
-// a value is read once.  Measured: 4096 x 4096 bf16 7.9 us and back 7.4 (42 MB each, 5.5
-// TB/s), fp32 weights [4096][8192] 25.6 (152 MB, 5.9 TB/s; operands that the caches held
+// a value is read once.  Measured: 4096 x 4096 bf16 8.0 us and back 7.4 (42 MB each, 5.3 and
+// 5.7 TB/s), fp32 weights [4096][8192] 23.2 (152 MB, 6.5 TB/s; operands that the caches held
 // from the call before), there and back with others each time 56; with a thread to a
 // block and its 32 values read one by one 166 and 749 there and back.
 #include <type_traits>

@@ -4,9 +4,11 @@
 // consecutive columns of one row of C.
 //
 // k_mxmm_few: tiles of 16, 32 or 64 on the 16 x 16 x 128 MFMA, K split between a
-// workgroup's waves.  A launch's latency bounds the smallest, the reading of the weights
-// the others: 1 x 4096 x 4096 3.5 us in a graph with the quantization of its row, 1 x
-// 16384 -> 4096 8.4 (34 MB, 4 TB/s), 128 x 8192 x 4096 6.7.
+// workgroup's waves.  A launch's latency bounds the smallest, the latency of loads the
+// others, of which a wave has one unit under way at a time.  In a graph, us: 1 x 4096 x
+// 4096 with the quantization of its row 3.4 on the same operands, 4.4 with weights from
+// HBM; 1 x 16384 -> 4096 7.1 and 10.7 (34 MB, 3.2 TB/s); the product 128 x 8192 x 4096 6.9
+// and 9.2.
 //
 // k_mxmm: four waves of 2 x 2 or 4 x 4 blocks of 32 x 32, operands DMA'd into LDS in
 // chunks of 128 k, four stages.  The 256 x 256 tile needs 512 bytes of LDS reads per
@@ -200,6 +202,8 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
         else quantize(std::integral_constant<int, 2>{});
         __syncthreads();
     }
+    // (The copy makes the compiler wait for all of r at the end of a turn: the next unit's
+    // loads overlap with this unit's MFMAs, and no more than one unit is under way.)
     for (unsigned i = 0; u < units;) {
         Unit c = r;
         const unsigned v = unit(++i);

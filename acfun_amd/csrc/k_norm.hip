@@ -13,8 +13,12 @@
 // residual of 8192 x 8192 bf16 97 us (537 MB, 5.5 TB/s, a copy's rate), the norm of
 // 4096 x 4096 fp16 12.3 us; one token 2.1 and eight 3.9 us in a graph, 4.1 and 4.7 from
 // the host, which is the cost of a launch.  Rows whose width is no whole chunk start
-// off a dword's boundary in 16-bit types: 8192 x 8111 135 us.  With a value per thread
-// and step and parameters read for every row: 478, 26.1, 5.6 and 21.2.
+// off a dword's boundary in 16-bit types: 8192 x 8111 137 us (3.9 TB/s).  With a value per
+// thread and step and parameters read for every row: 478, 26.1, 5.6 and 21.2.
+// Wide rows, norm and residual, TB/s: 8192 x 16384 bf16 5.5, 4096 x 32768 bf16 4.7; fp32 4096
+// x 16384 5.0, 4096 x 32768 4.5; the norm alone 5.3 to 5.8.  The least are widths just past
+// a launch's step, which leave up to half of the threads without a chunk: 8192 x 8448 bf16
+// 4.2, 4096 x 16388 fp32 3.8.
 #include <type_traits>
 
 #include "mx.hpp"
@@ -57,10 +61,13 @@ struct RowSum {
 // TPR threads to a row (64: a wave, four rows to a workgroup), CH chunks of 16
 // bytes to a thread.  The row stays in registers, so every value is read once;
 // a workgroup takes rows in turn, `step` apart.  With one or two chunks it keeps the
-// weights and the gate of its columns and has the next row's loads under way (128
-// registers hold that, for four waves per SIMD); biases are read where they are
-// added.  WHOLE: rows are whole chunks, so a thread's chunk is all there or not at
-// all, with half the code: one row's time is for a good part the fetching of it.
+// weights and the gate of its columns and has the next row's loads under way; biases
+// are read where they are added.  128 registers, for four waves per SIMD, hold that
+// but for some residuals past 8192 columns: 2 registers of a lane go to memory with
+// 1024 threads and two chunks of 16-bit types, 2 with four chunks of fp16 in rows of no
+// whole chunk, and 44 to 48 with the eight chunks of fp32 past 16384 columns.  WHOLE: rows
+// are whole chunks, so a thread's chunk is all there or not at all, with half the code:
+// one row's time is for a good part the fetching of it.
 // (gridDim is not asked for: the hidden arguments that it comes with, and any more
 // than 128 bytes of them, cost a launch 0.7 us on the host.)
 template <class T, int TPR, int CH, bool RES, bool WHOLE>

@@ -47,12 +47,13 @@ constexpr bool mm_fits(int M, int N, int K) {
 }
 
 // Times in us that choose a kernel and its tile, fitted to those of every tile over
-// 546 sizes (M of 16 to 8192, N of 64 to 8192, K of 128 to 8192; bf16, replayed from a
-// graph): a call takes `lat` while the CUs have less than a tile each, and `base` and
-// `each` times the tiles of a CU from there.  The tile chosen is 0.8 % slower than the
-// best of each size in the mean.  Measured, us: 128 x 8192 x 4096 9.4 with tiles of 32,
-// 8.0 with 64, 11.0 with 128; 512 x 8192 x 1024 14.2 with 64, 6.7 with 128; 8192 x 8192 x
-// 4096 154 with 128, 136 with 256 (other operands each time).
+// 300 sizes (bf16, replayed from a graph): a call takes `lat` while the CUs have less
+// than a tile each, and `base` and `each` times the tiles of a CU from there.  Over 360
+// sizes (M of 16 to 8192, N of 64 to 8192, K of 128 to 8192, three sets of operands in
+// turn) the tile chosen is 0.8 % slower than the best of each in the mean, 25 % at most
+// (64 x 2048 x 8192: 7.2 with tiles of 32, 5.7 with 16).  Measured, us: 128 x 8192 x 4096
+// 10.0 with tiles of 32, 8.6 with 64, 11.1 with 128; 512 x 8192 x 1024 14.6 with 64, 6.8
+// with 128; 8192 x 8192 x 4096 154 with 128, 132 with 256.
 inline double tile_time(double lat, double base, double each, double tiles_per_cu) {
     const double t = base + each * tiles_per_cu;
     return t > lat ? t : lat;
@@ -113,9 +114,8 @@ constexpr bool fc_fits(int M, int N, int K) {
 // The rows up to which a layer is always one launch while its stream is captured into a
 // graph, where LDS has room for 16 of them: two launches need a temporary, which a graph
 // cannot keep, and programs that capture have to know beforehand what they may.  Measured
-// in a graph, us, against two calls on the caller's buffers: 16 x 4096 x 4096 6.4 and 5.6,
-// 128 x 4096 x 4096 10.7 and 9.4, 512 x 4096 x 4096 35.6 and 15.4, 512 x 8192 x 8192 196
-// and 26.
+// in a graph, us, against two calls on the caller's buffers: 16 x 4096 x 4096 5.8 and 5.1,
+// 128 x 4096 x 4096 10.0 and 8.9, 512 x 4096 x 4096 34 and 15, 512 x 8192 x 8192 196 and 27.
 constexpr int kCapturedRows = 512;
 
 struct FcPlan {

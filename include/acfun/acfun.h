@@ -310,7 +310,8 @@ void acfun_fc_mxfp4(const float* input, int N, int Cin, const uint8_t* weight, c
 /* Norms of rows (at most 32768 columns):
  *   ACFUN_RMSNORM    norm(v) = v / sqrt(mean(v^2) + eps) * weight + bias
  *   ACFUN_LAYERNORM  norm(v) = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias
- * with weight and bias [cols], NULL meaning 1 and 0. */
+ * with weight and bias [cols], NULL meaning 1 and 0.  The sum of squares is in fp32: a
+ * row whose sum passes its range (values past 1.8e19) has v taken times 0. */
 #define ACFUN_RMSNORM 0
 #define ACFUN_LAYERNORM 1
 
