@@ -29,9 +29,9 @@ def test_kinds(tmp_path):
     assert mx_plans.ask(exe, [mx_plans.gemm(*p[:3]) for p in two]) == [p[4] for p in two]
 
 
-def _shift(n, K, t):
-    """(scale bytes about) 1 for fp32 and bf16; for fp16 as far below as keeps sums in its range."""
-    return n if t != "f16" else np.minimum(n, 124) - 12
+def _scales(byte, t):
+    """A's scale bytes; for fp16 so far below 1 that the sums stay in its range."""
+    return byte if t != "f16" else np.minimum(byte, 124) - 12
 
 
 @pytest.mark.gpu
@@ -43,7 +43,7 @@ def test_product(gpu, rng, i, t):
     M, N, K, _ = PRODUCTS[i]
     n = i + NAMES.index(t)
     a, b = _operand(rng, M, K, 3), _operand(rng, N, K, 3)
-    a = (a[0], _shift(a[1], K, t))
+    a = (a[0], _scales(a[1], t))
     bias = rng.standard_normal(N).astype(np.float32) if n % 3 != 1 else None
     act = int(n % 3 == 0)
     got = _gemm(gpu, a, b, bias, act, t, M, N, K)
