@@ -86,6 +86,19 @@ SIGNATURES = {
     "acfun_dev_fc_mxfp4": (_i, [_p, _i, _i, _i, _p, _p, _p, _i, _p, _i, _p]),
     "acfun_quantize_weights_mxfp4": (None, [_p, _i, _i, _p, _p]),
     "acfun_fc_mxfp4": (None, [_p, _i, _i, _p, _p, _p, _i, _p, _i]),
+    "acfun_q8_code_bytes": (_sz, [_i, _i]),
+    "acfun_q8_scale_bytes": (_sz, [_i]),
+    "acfun_dev_quantize_q8": (_i, [_p, _i, _i, _i, _i, _p, _p, _p]),
+    "acfun_dev_dequantize_q8": (_i, [_p, _p, _i, _i, _p, _i, _p]),
+    "acfun_dev_gemm_q8": (_i, [_i, _i, _i, _p, _p, _p, _p, _p, _i, _p, _i, _p]),
+    "acfun_dev_fc_q8": (_i, [_p, _i, _i, _i, _p, _p, _p, _i, _p, _i, _p]),
+    "acfun_dev_gemm_gated_q8": (_i, [_i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _i, _p, _p, _i, _p]),
+    "acfun_dev_fc_gated_q8": (_i, [_p, _i, _i, _i, _p, _p, _p, _p, _p, _p, _i, _p, _i, _p]),
+    "acfun_quantize_weights_q8": (None, [_p, _i, _i, _p, _p]),
+    "acfun_fc_q8": (None, [_p, _i, _i, _p, _p, _p, _i, _p, _i]),
+    "acfun_fc_gated_q8": (None, [_p, _i, _i, _p, _p, _p, _p, _p, _p, _i, _p, _i]),
+    "acfun_dev_sample": (_i, [_p, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "acfun_sample": (None, [_p, _i, _i, _p, _p, _p, _p, _p, _p, _p]),
     "acfun_dev_norm": (_i, [_p, _i, _i, _i, _i, _p, _p, _f, _p, _p]),
     "acfun_dev_norm_residual": (_i, [_p, _p, _i, _i, _i, _i, _p, _p, _p, _i, _f, _p, _p, _f, _p,
                                      _p, _p]),

@@ -1,11 +1,12 @@
 // capi_block.cpp -- the extern "C" entry points for transformer layers
-// (include/acfun/acfun.h): MXFP4 quantizer and products, norms around a block.
+// (include/acfun/acfun.h): MXFP4 and Q8 quantizers and products, norms around a block,
+// sampling.
 // Arguments are checked before the device is touched; nothing is written when
 // a call is refused, and no C++ exception leaves an entry.
 #include <exception>
 
 #include "../../include/acfun/acfun.h"
-#include "mx.hpp"
+#include "q8.hpp"
 
 using namespace acfun;
 
@@ -39,8 +40,9 @@ struct Checks {
         return out == in ? *this : apart(out, n, in, n);
     }
     Checks& param(const float* p) { return need((uintptr_t)p % 4 == 0, "a parameter is not aligned to 4 bytes"); }
+    Checks& param(const int* p) { return param((const float*)p); }
     Checks& fits(bool f) { return need(f, "too large: a launch holds fewer than 2^32 threads"); }
-    Checks& held(const uint8_t* codes, const uint8_t* scales) {
+    Checks& held(const void* codes, const void* scales) {
         need(codes && scales, "codes or scales are NULL");
         return need((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0,
                     "codes or scales are not aligned to 16 bytes");
@@ -71,6 +73,53 @@ void staged(const char* who, F f) {
             return false;
         }
         return hc.finish();
+    });
+}
+
+// A product of Q8 operands, or (rows) a layer on float rows.
+int q8_product(const char* who, const Q8Product& p, int type, bool rows, void* stream) {
+    Checks c{who};
+    c.type(type).need(p.act >= 0 && p.act <= ACFUN_GELU_TANH, "act is not 0 or one of ACFUN_RELU to ACFUN_GELU_TANH");
+    if (!c.need(p.M >= 0 && p.N >= 0 && p.K >= 0, "a size is negative").ok) return -1;
+    if (p.M == 0 || p.N == 0) return 0;
+    c.need(p.K <= kQ8MaxK, "K is more than 131072: sums of products could pass 32 bits");
+    const int mats = p.gated ? 2 : 1;
+    const size_t n = (size_t)p.M * p.N * type_size(type);
+    if (p.K > 0) {
+        if (rows) c.tensor(p.A, type, "input is NULL");
+        else c.held(p.A, p.As);
+        for (int g = 0; g < mats; ++g) c.held(p.B[g], p.Bs[g]);
+    }
+    c.tensor(p.C, type, "the result is NULL");
+    for (int g = 0; g < mats; ++g) c.param(p.bias[g]);
+    if (!c.ok) return -1;
+    if (p.K > 0) {
+        if (rows) c.apart(p.C, n, p.A, (size_t)p.M * p.K * type_size(type));
+        else c.apart(p.C, n, p.A, q8_code_bytes(p.M, p.K)).apart(p.C, n, p.As, q8_scale_bytes(p.M));
+        for (int g = 0; g < mats; ++g)
+            c.apart(p.C, n, p.B[g], q8_code_bytes(p.N, p.K)).apart(p.C, n, p.Bs[g], q8_scale_bytes(p.N));
+    }
+    for (int g = 0; g < mats; ++g) c.apart(p.C, n, p.bias[g], 4 * (size_t)p.N);
+    if (!c.fits(q8_mm_fits(p.M, p.N) && (!rows || q8_quant_fits(p.M, 0))).ok) return -1;
+    return call(who, [&] { return rows ? q8_fc(who, p, type, resolve(stream)) : q8_gemm(p, type, resolve(stream)); });
+}
+
+// A layer on host or device pointers, fp32.
+void q8_host_layer(Checks c, Q8Product p) {
+    if (p.M <= 0 || p.K < 0 || p.N <= 0) return;
+    const int mats = p.gated ? 2 : 1;
+    c.need(p.C && (p.K == 0 || p.A), "a pointer is NULL");
+    for (int g = 0; g < mats; ++g) c.need(p.K == 0 || (p.B[g] && p.Bs[g]), "a pointer is NULL");
+    if (!c.ok) return;
+    staged(c.who, [&](HostCall& hc) {
+        p.A = hc.in(p.A, (size_t)p.M * p.K * sizeof(float));
+        for (int g = 0; g < mats; ++g) {
+            p.B[g] = (const int8_t*)hc.in(p.B[g], acfun_q8_code_bytes(p.N, p.K));
+            p.Bs[g] = (const float*)hc.in(p.Bs[g], q8_scale_bytes(p.N));
+            p.bias[g] = (const float*)hc.in(p.bias[g], (size_t)p.N * sizeof(float));
+        }
+        p.C = hc.out(p.C, (size_t)p.M * p.N * sizeof(float));
+        return !hc.failed() && q8_product(c.who, p, ACFUN_F32, true, hc.stream()) == 0;
     });
 }
 
@@ -168,6 +217,132 @@ void acfun_fc_mxfp4(const float* input, int N, int Cin, const uint8_t* weight, c
         auto dy = (float*)hc.out(output, (size_t)N * Cout * sizeof(float));
         return !hc.failed() &&
                acfun_dev_fc_mxfp4(dx, ACFUN_F32, N, Cin, dw, ds, db, Cout, dy, act, hc.stream()) == 0;
+    });
+}
+
+// ------------------------------------------------------------------ Q8
+size_t acfun_q8_code_bytes(int rows, int K) { return rows > 0 && K > 0 ? q8_code_bytes(rows, K) : 0; }
+size_t acfun_q8_scale_bytes(int rows) { return rows > 0 ? q8_scale_bytes(rows) : 0; }
+
+int acfun_dev_quantize_q8(const void* x, int type, int rows, int K, int trans, int8_t* codes, float* scales,
+                          void* stream) {
+    Checks c{"acfun_dev_quantize_q8"};
+    if (!c.type(type).need(rows >= 0 && K >= 0, "a size is negative").ok) return -1;
+    if (rows == 0 || K == 0) return 0;
+    if (!c.tensor(x, type, "x is NULL").held(codes, scales).ok) return -1;
+    const size_t n = (size_t)rows * K * type_size(type);
+    c.apart(codes, q8_code_bytes(rows, K), x, n).apart(scales, q8_scale_bytes(rows), x, n);
+    c.apart(codes, q8_code_bytes(rows, K), scales, q8_scale_bytes(rows));
+    if (!c.fits(q8_quant_fits(rows, trans)).ok) return -1;
+    return call(c.who, [&] { return q8_quantize(x, type, rows, K, trans, codes, scales, resolve(stream)); });
+}
+
+int acfun_dev_dequantize_q8(const int8_t* codes, const float* scales, int rows, int K, void* x, int type,
+                            void* stream) {
+    Checks c{"acfun_dev_dequantize_q8"};
+    if (!c.type(type).need(rows >= 0 && K >= 0, "a size is negative").ok) return -1;
+    if (rows == 0 || K == 0) return 0;
+    if (!c.tensor(x, type, "x is NULL").held(codes, scales).ok) return -1;
+    const size_t n = (size_t)rows * K * type_size(type);
+    if (!c.apart(x, n, codes, q8_code_bytes(rows, K)).apart(x, n, scales, q8_scale_bytes(rows)).ok) return -1;
+    if (!c.fits(q8_dequant_fits(rows, K)).ok) return -1;
+    return call(c.who, [&] { return q8_dequantize(codes, scales, rows, K, x, type, resolve(stream)); });
+}
+
+int acfun_dev_gemm_q8(int M, int N, int K, const int8_t* A, const float* a_scales, const int8_t* B,
+                      const float* b_scales, void* C, int type, const float* bias, int act, void* stream) {
+    return q8_product("acfun_dev_gemm_q8", {M, N, K, A, a_scales, {B}, {b_scales}, {bias}, C, act, false}, type, false,
+                      stream);
+}
+
+int acfun_dev_fc_q8(const void* input, int type, int N, int Cin, const int8_t* weight, const float* wscale,
+                    const float* bias, int Cout, void* output, int act, void* stream) {
+    return q8_product("acfun_dev_fc_q8", {N, Cout, Cin, input, nullptr, {weight}, {wscale}, {bias}, output, act, false},
+                      type, true, stream);
+}
+
+int acfun_dev_gemm_gated_q8(int M, int N, int K, const int8_t* A, const float* a_scales, const int8_t* G,
+                            const float* g_scales, const int8_t* U, const float* u_scales, void* C, int type,
+                            const float* gbias, const float* ubias, int act, void* stream) {
+    return q8_product("acfun_dev_gemm_gated_q8",
+                      {M, N, K, A, a_scales, {G, U}, {g_scales, u_scales}, {gbias, ubias}, C, act, true}, type, false,
+                      stream);
+}
+
+int acfun_dev_fc_gated_q8(const void* input, int type, int N, int Cin, const int8_t* gate, const float* gscale,
+                          const float* gbias, const int8_t* up, const float* uscale, const float* ubias, int Cout,
+                          void* output, int act, void* stream) {
+    return q8_product("acfun_dev_fc_gated_q8",
+                      {N, Cout, Cin, input, nullptr, {gate, up}, {gscale, uscale}, {gbias, ubias}, output, act, true},
+                      type, true, stream);
+}
+
+void acfun_quantize_weights_q8(const float* w, int K, int N, int8_t* codes, float* scales) {
+    if (K <= 0 || N <= 0) return;
+    Checks c{"acfun_quantize_weights_q8"};
+    if (!c.need(w && codes && scales, "a pointer is NULL").ok) return;
+    staged(c.who, [&](HostCall& hc) {
+        auto dw = (const float*)hc.in(w, (size_t)K * N * sizeof(float));
+        auto dc = (int8_t*)hc.out(codes, q8_code_bytes(N, K));
+        auto ds = (float*)hc.out(scales, q8_scale_bytes(N));
+        return !hc.failed() && acfun_dev_quantize_q8(dw, ACFUN_F32, N, K, 1, dc, ds, hc.stream()) == 0;
+    });
+}
+
+void acfun_fc_q8(const float* input, int N, int Cin, const int8_t* weight, const float* wscale, const float* bias,
+                 int Cout, float* output, int act) {
+    q8_host_layer({"acfun_fc_q8"}, {N, Cout, Cin, input, nullptr, {weight}, {wscale}, {bias}, output, act, false});
+}
+
+void acfun_fc_gated_q8(const float* input, int N, int Cin, const int8_t* gate, const float* gscale,
+                       const float* gbias, const int8_t* up, const float* uscale, const float* ubias, int Cout,
+                       float* output, int act) {
+    q8_host_layer({"acfun_fc_gated_q8"},
+                  {N, Cout, Cin, input, nullptr, {gate, up}, {gscale, uscale}, {gbias, ubias}, output, act, true});
+}
+
+// ------------------------------------------------------------------ sampling
+int acfun_dev_sample(const void* logits, int type, int rows, int cols, int ld, const float* temperature,
+                     const int* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
+                     float* prob, void* stream) {
+    Checks c{"acfun_dev_sample"};
+    if (!c.type(type).need(rows >= 0 && cols >= 0, "a size is negative").need(ld >= cols, "ld is less than cols").ok)
+        return -1;
+    if (rows == 0) return 0;
+    c.need(cols <= kSampleMaxCols, "more than 2^24 columns").fits(sample_fits(rows));
+    if (cols > 0) c.tensor(logits, type, "logits is NULL");
+    c.need(u != nullptr, "u is NULL").need(token != nullptr, "token is NULL");
+    c.param(temperature).param(top_k).param(top_p).param(min_p).param(u).param(token).param(prob);
+    if (!c.ok) return -1;
+    const size_t n = cols > 0 ? ((size_t)(rows - 1) * ld + cols) * type_size(type) : 0, np = 4 * (size_t)rows;
+    c.apart(token, np, prob, np);
+    for (const void* out : {(const void*)token, (const void*)prob}) {
+        if (!out) continue;
+        c.apart(out, np, logits, n);
+        for (const void* in : {(const void*)temperature, (const void*)top_k, (const void*)top_p, (const void*)min_p,
+                               (const void*)u})
+            c.apart(out, np, in, np);
+    }
+    if (!c.ok) return -1;
+    const SampleArgs a{logits, rows, cols, ld, temperature, top_k, top_p, min_p, u, token, prob};
+    return call(c.who, [&] { return sample_rows(a, type, resolve(stream)); });
+}
+
+void acfun_sample(const float* logits, int rows, int cols, const float* temperature, const int* top_k,
+                  const float* top_p, const float* min_p, const float* u, int32_t* token, float* prob) {
+    if (rows <= 0 || cols < 0) return;
+    Checks c{"acfun_sample"};
+    if (!c.need((cols == 0 || logits) && u && token, "a pointer is NULL").ok) return;
+    staged(c.who, [&](HostCall& hc) {
+        const size_t n = 4 * (size_t)rows;
+        auto dx = (const float*)hc.in(logits, n * cols);
+        auto dt = (const float*)hc.in(temperature, n);
+        auto dk = (const int*)hc.in(top_k, n);
+        auto dp = (const float*)hc.in(top_p, n), dm = (const float*)hc.in(min_p, n), du = (const float*)hc.in(u, n);
+        auto to = (int32_t*)hc.out(token, n);
+        auto pr = (float*)hc.out(prob, n);
+        return !hc.failed() &&
+               acfun_dev_sample(dx, ACFUN_F32, rows, cols, cols, dt, dk, dp, dm, du, to, pr, hc.stream()) == 0;
     });
 }
 

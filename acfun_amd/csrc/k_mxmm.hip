@@ -20,8 +20,8 @@
 // that its 67 MB of results are stored at once, at the end); with a wave to each 16 x
 // 16 of C and operands from memory 1,800 and 190.
 #include <type_traits>
-#include <utility>
 
+#include "mm.hpp"
 #include "mx.hpp"
 
 namespace acfun {
@@ -32,29 +32,8 @@ typedef int i8v __attribute__((ext_vector_type(8)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void lds_void;
 
 __device__ __forceinline__ i8v wide(i4v v) { return i8v{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
-
-// f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>)
-template <class F, int... I>
-__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, class F>
-__device__ __forceinline__ void each(F f) { each_of(f, std::make_integer_sequence<int, N>{}); }
-
-// XCD x (workgroup id mod 8) owns a contiguous run of the `total` tiles: the number
-// of this workgroup's, or `total` if it has none.
-__device__ __forceinline__ unsigned xcd_tile(unsigned total) {
-    const unsigned x = blockIdx.x & 7;
-    auto first = [&](unsigned y) { return y * (total >> 3) + (y * (total & 7) >> 3); };
-    const unsigned l = first(x) + (blockIdx.x >> 3);
-    return l < first(x + 1) ? l : total;
-}
-
-// ReLU where lo is 0, nothing where it is -infinity; NaN stays NaN.
-__device__ __forceinline__ float at_least(float v, float lo) { return __builtin_elementwise_maximum(v, lo); }
 
 struct MmArgs {
     int M, N, K;
@@ -256,21 +235,6 @@ __global__ __launch_bounds__(64 * W) void k_mxmm_few(MmArgs p) {
 }
 
 // ---------------------------------------------------------------- many rows
-// s_waitcnt vmcnt(n), n < 64
-constexpr int mx_vmcnt(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
-
-// 64 times 16 (or 4) bytes from q into LDS; nothing is read unless `live`.
-__device__ __forceinline__ void mx_dma16(const uint8_t* q, bool live, char* lds, unsigned voff, unsigned soff) {
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc((void*)q, (short)0, live ? 0x7fffffff : 0, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds, 16, voff, soff, 0, 0);
-}
-__device__ __forceinline__ void mx_dma4(const uint8_t* q, bool live, char* lds, unsigned voff, unsigned soff) {
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc((void*)q, (short)0, live ? 0x7fffffff : 0, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds, 4, voff, soff, 0, 0);
-}
-
 template <int FM, int FN>
 struct MmTile {
     static constexpr int BM = 64 * FM, BN = 64 * FN;        // 2 x 2 waves of FM x FN blocks of 32 x 32
@@ -319,13 +283,13 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void k_mxmm(MmArgs p) {
         constexpr int t = decltype(tile)::value;
         const bool live = g < st;
         char* const to = smx + 4 * Tl::STG + g % 3 * Tl::SCL + wave * 256;
-        mx_dma4(t < FM ? As0 : Bs0, live, to + t * 1024, lane * 4, os[t] + (live ? g : 0) * 256u);
+        lds_dma4(t < FM ? As0 : Bs0, live, to + t * 1024, lane * 4, os[t] + (live ? g : 0) * 256u);
     };
     auto codes = [&](int c, int stage, auto tile) {
         constexpr int t = decltype(tile)::value;
         const bool live = c < kt;
         char* const to = smx + stage * Tl::STG + wave * 1024;
-        mx_dma16(t < FM ? A0 : B0, live, to + t * 4096, lane * 16, oc[t] + (live ? c : 0) * 1024u);
+        lds_dma16(t < FM ? A0 : B0, live, to + t * 4096, lane * 16, oc[t] + (live ? c : 0) * 1024u);
     };
     auto issue = [&](int c, auto stage, auto item) {
         constexpr int t = decltype(item)::value, q = decltype(stage)::value;
@@ -405,7 +369,7 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void k_mxmm(MmArgs p) {
         each<SI>([&](auto i) { scales(1, i); });
     }
     each<H1>([&](auto i) { codes(3, 3, i); });
-    __builtin_amdgcn_s_waitcnt(mx_vmcnt(2 * ITEMS + H1));
+    __builtin_amdgcn_s_waitcnt(vm_count(2 * ITEMS + H1));
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     each<CI>([&](auto i) { read_scale(0, Zero{}, i); });
     each<CI>([&](auto i) { read(Zero{}, Zero{}, i); });
@@ -424,7 +388,7 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void k_mxmm(MmArgs p) {
             constexpr int q = decltype(Q)::value;
             if (q > 0 && c + q >= kt) return;
             half(c + q, Q, Zero{});
-            __builtin_amdgcn_s_waitcnt(mx_vmcnt(2 * ITEMS));
+            __builtin_amdgcn_s_waitcnt(vm_count(2 * ITEMS));
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             half(c + q, Q, One{});
         });
@@ -433,7 +397,7 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void k_mxmm(MmArgs p) {
     // Lane l, register e of a block: row l % 32, column 8 (e / 4) + 4 (l / 32) + e % 4.
     // A wave turns its results around in LDS, for stores of
     // whole cache lines.  16 bytes between rows: 8 lanes' writes fall on different banks.
-    __builtin_amdgcn_s_waitcnt(mx_vmcnt(0));                // the chunks past the end
+    __builtin_amdgcn_s_waitcnt(vm_count(0));                // the chunks past the end
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (p.bias) {
         // an fp32 MFMA of the bias and 1 (one of its two k is 0): exact

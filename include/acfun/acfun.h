@@ -307,6 +307,96 @@ void acfun_quantize_weights_mxfp4(const float* w, int K, int N, uint8_t* codes, 
 void acfun_fc_mxfp4(const float* input, int N, int Cin, const uint8_t* weight, const uint8_t* wscale,
                     const float* bias, int Cout, float* output, int act);
 
+/* 8-bit integers with a scale for each row (Q8): with a = max|x| of the row, scale =
+ * a / 127 in fp32 and each code x / scale rounded to the nearest integer, halves to the
+ * even one.  A row whose scale would be below 2^-126 is zeros with scale 0; a row with a
+ * NaN or an infinity has scale NaN and codes 0, and stands for NaN.  Weights as rows
+ * have a scale for each output channel, activations one for each token.
+ *
+ * An operand of `rows` rows is two arrays, each aligned to 16 bytes (rows padded to 16,
+ * K to 64, with zeros):
+ *   codes   tiles of 16 rows x 64 k, row tiles outermost, 1024 bytes each: byte
+ *           (16 j + r) * 16 + i of a tile holds k = 16 j + i of row r;
+ *   scales  one fp32 for each row.
+ * The sizes of the arrays in bytes (0 for an empty operand): */
+size_t acfun_q8_code_bytes(int rows, int K);
+size_t acfun_q8_scale_bytes(int rows);
+
+/* x [rows, K] (trans 0) or [K, rows] (trans 1: weights as acfun_fc takes them,
+ * rows = Cout) -> an operand, with a scale for each of the `rows` either way. */
+int acfun_dev_quantize_q8(const void* x, int type, int rows, int K, int trans, int8_t* codes, float* scales,
+                          void* stream);
+/* The values an operand stands for, as x [rows, K]; at most the largest of `type` where
+ * the scale is finite (127 times a rounded scale may pass the largest fp32). */
+int acfun_dev_dequantize_q8(const int8_t* codes, const float* scales, int rows, int K, void* x, int type,
+                            void* stream);
+
+/* Activations (`act`) of the calls below; 0 is none.  NaN stays NaN. */
+#define ACFUN_RELU 1       /* max(v, 0) */
+#define ACFUN_SILU 2       /* v / (1 + exp(-v)) */
+#define ACFUN_GELU 3       /* v (1 + erf(v / sqrt 2)) / 2 */
+#define ACFUN_GELU_TANH 4  /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+
+/* C[M,N] = act(A * B^T + bias[n]) (bias NULL = none), A an operand of M rows, B of N rows;
+ * C of `type`.  Sums are exact (32-bit integers, for which K is at most 131072) and
+ * become (sum * A's scale) * B's scale in fp32, whatever the sizes: a row's result does
+ * not depend on the other rows of its call.  K = 0 gives act(bias). */
+int acfun_dev_gemm_q8(int M, int N, int K, const int8_t* A, const float* a_scales, const int8_t* B,
+                      const float* b_scales, void* C, int type, const float* bias, int act, void* stream);
+/* A fully connected layer with weights held in Q8 (an operand of Cout rows): input
+ * [N, Cin] is quantized as acfun_dev_quantize_q8 does and multiplied; output [N, Cout].
+ * Input and output are of `type`.  The call is one launch without temporaries, or two with
+ * the quantized input in the library's pool; the results are the same bits.  On a stream
+ * that is being captured into a graph it is one launch for N of at most 512 and Cin of at
+ * most 8192 (131072 for N = 1); past that it may be refused: quantize into buffers of the
+ * caller's and multiply, which can be captured at any size. */
+int acfun_dev_fc_q8(const void* input, int type, int N, int Cin, const int8_t* weight, const float* wscale,
+                    const float* bias, int Cout, void* output, int act, void* stream);
+
+/* The gated half of a feed-forward block, two projections of the same rows:
+ *   C[M,N] = act(A * G^T + gbias[n]) * (A * U^T + ubias[n])
+ * (ACFUN_SILU, ACFUN_GELU, ACFUN_RELU, or 0 for the plain product of the two), with G and
+ * U operands of N rows.  Neither projection is rounded or stored. */
+int acfun_dev_gemm_gated_q8(int M, int N, int K, const int8_t* A, const float* a_scales, const int8_t* G,
+                            const float* g_scales, const int8_t* U, const float* u_scales, void* C, int type,
+                            const float* gbias, const float* ubias, int act, void* stream);
+/* The same on float rows, as acfun_dev_fc_q8: launches and graphs are as there. */
+int acfun_dev_fc_gated_q8(const void* input, int type, int N, int Cin, const int8_t* gate, const float* gscale,
+                          const float* gbias, const int8_t* up, const float* uscale, const float* ubias, int Cout,
+                          void* output, int act, void* stream);
+/* The same on host or device pointers, synchronous, fp32: weights w [K, N] into an
+ * operand of N rows, the layer, and the gated layer. */
+void acfun_quantize_weights_q8(const float* w, int K, int N, int8_t* codes, float* scales);
+void acfun_fc_q8(const float* input, int N, int Cin, const int8_t* weight, const float* wscale, const float* bias,
+                 int Cout, float* output, int act);
+void acfun_fc_gated_q8(const float* input, int N, int Cin, const int8_t* gate, const float* gscale,
+                       const float* gbias, const int8_t* up, const float* uscale, const float* ubias, int Cout,
+                       float* output, int act);
+
+/* A token for each of `rows` rows of logits [rows, cols], whose rows start ld elements
+ * apart (ld >= cols; at most 2^24 columns).  A row is drawn from as follows:
+ *   w_i = exp((x_i - max x) / temperature); -infinity and NaN are never drawn;
+ *   tokens are in order of x, the lowest index first of equal ones, and kept are
+ *   the first top_k of them (0 or less: all),
+ *   of these the fewest of the order whose weights reach top_p of theirs, at least one
+ *   (1 or more: all),
+ *   of these the ones with w_i >= min_p (0 or less: all; past 1: as 1);
+ *   token = the first kept i, in order of index, with sum of w_j over j <= i  >  u * sum.
+ * A temperature of 0 or less takes the largest x, the lowest index of equal ones.  Each of
+ * temperature, top_k, top_p and min_p is an array [rows] or NULL (1 and off), and a NaN in one
+ * turns it off (a temperature: 0).  Beside a logit of +infinity finite ones have weight 0.
+ * u [rows] are the caller's random numbers in [0, 1); others are taken to its ends, 0 (and a
+ * NaN) and 1 - 2^-24.  token [rows] gets the index, -1 for a row with nothing to draw,
+ * and prob [rows] (NULL: not wanted) the probability it was drawn with, 0 for -1.
+ * Sums of weights are in integers of 64 bits and the same in any order, so that a row's
+ * token does not depend on the other rows or on the launch. */
+int acfun_dev_sample(const void* logits, int type, int rows, int cols, int ld, const float* temperature,
+                     const int* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
+                     float* prob, void* stream);
+/* The same on host or device pointers, synchronous, fp32, ld = cols. */
+void acfun_sample(const float* logits, int rows, int cols, const float* temperature, const int* top_k,
+                  const float* top_p, const float* min_p, const float* u, int32_t* token, float* prob);
+
 /* Norms of rows (at most 32768 columns):
  *   ACFUN_RMSNORM    norm(v) = v / sqrt(mean(v^2) + eps) * weight + bias
  *   ACFUN_LAYERNORM  norm(v) = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias
