@@ -100,7 +100,7 @@ int q8_product(const char* who, const Q8Product& p, int type, bool rows, void* s
             c.apart(p.C, n, p.B[g], q8_code_bytes(p.N, p.K)).apart(p.C, n, p.Bs[g], q8_scale_bytes(p.N));
     }
     for (int g = 0; g < mats; ++g) c.apart(p.C, n, p.bias[g], 4 * (size_t)p.N);
-    if (!c.fits(q8_mm_fits(p.M, p.N) && (!rows || q8_quant_fits(p.M, 0))).ok) return -1;
+    if (!c.fits(q8_mm_fits(p.M, p.N, p.K, p.gated) && (!rows || q8_quant_fits(p.M, 0))).ok) return -1;
     return call(who, [&] { return rows ? q8_fc(who, p, type, resolve(stream)) : q8_gemm(p, type, resolve(stream)); });
 }
 

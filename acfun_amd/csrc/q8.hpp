@@ -20,26 +20,98 @@ namespace acfun {
 // The scale of a row from the bits of its max|x| (fp32, no sign), and what its
 // codes are found with.
 struct Q8Scale {
-    float s, inv;
-    bool codes;                                 // false: they are all 0
+    float s, inv;                               // inv 0: codes are all 0
+    Q8Scale() = default;
     __device__ __forceinline__ explicit Q8Scale(unsigned top) {
         s = __uint_as_float(top) / 127.f;
-        codes = s >= 0x1p-126f && top < 0x7f800000u;
-        if (top >= 0x7f800000u) s = __uint_as_float(0x7fc00000u);
-        else if (!codes) s = 0.f;
-        inv = 1.f / s;
-    }
-    // x / s rounded, halves to even.  x times 1 / s is off by less than one; what is left
-    // over, x - q s, is a multiple of half of s's last place and no more than s, so the fused
-    // product has it exactly, and it says which side of the half x is on.
-    __device__ __forceinline__ int code(float x) const {
-        const float q = __builtin_rintf(x * inv), r = __builtin_fmaf(-q, s, x), t = 2.f * __builtin_fabsf(r);
-        const int i = (int)q, d = (int)(__float_as_uint(r) >> 31) * -2 + 1;
-        return codes ? i + (t > s || (t == s && (i & 1)) ? d : 0) : 0;
+        const bool bad = top >= 0x7f800000u, live = s >= 0x1p-126f && !bad;
+        s = bad ? __uint_as_float(0x7fc00000u) : live ? s : 0.f;
+        inv = live ? __builtin_amdgcn_rcpf(s) : 0.f;    // (a step or two off, which the codes allow for)
     }
 };
+// N values' codes, of which the low byte of c holds each.  q is x / s rounded, from x times
+// about 1 / s, in the low bits of a float that has no others below 1; it is off by less
+// than one.  What is left over, r = x - q s, is a multiple of half of s's last place and no
+// more than s, so the fused product has it exactly, and while it is less than half of s
+// for every value the codes are right.  False where it is not: halves, and quotients that
+// 1 / s brought to the wrong side of one, a few in a million.
+constexpr float kQ8Round = 0x1.8p23f;
+template <int N>
+__device__ __forceinline__ bool q8_codes_near(const Q8Scale& sc, const float (&v)[N], unsigned (&c)[N]) {
+    float most = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float z = __builtin_fmaf(v[e], sc.inv, kQ8Round);
+        c[e] = __float_as_uint(z);
+        most = __builtin_fmaxf(most, __builtin_fabsf(__builtin_fmaf(kQ8Round - z, sc.s, v[e])));
+    }
+    return 2.f * most < sc.s;
+}
+// The same for every value: where 2 |r| - s, exact too, is past 0, or is 0 and q odd, the
+// code is the next one on r's side.
+template <int N>
+__device__ __forceinline__ void q8_codes_exact(const Q8Scale& sc, const float (&v)[N], unsigned (&c)[N]) {
+    const unsigned mask = sc.inv == 0.f ? 0u : ~0u;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float z = __builtin_fmaf(v[e], sc.inv, kQ8Round), r = __builtin_fmaf(kQ8Round - z, sc.s, v[e]);
+        const float over = __builtin_fmaf(2.f, __builtin_fabsf(r), -sc.s);
+        const unsigned q = __float_as_uint(z);
+        const bool next = (int)(__float_as_uint(over) + (q & 1)) > 0;
+        c[e] = (q + (next ? (unsigned)((int)__float_as_uint(r) >> 31 | 1) : 0u)) & mask;
+    }
+}
+template <int N>
+__device__ __forceinline__ void q8_codes(const Q8Scale& sc, const float (&v)[N], unsigned (&c)[N]) {
+    if (!q8_codes_near(sc, v, c)) q8_codes_exact(sc, v, c);
+}
+// The low bytes of four.
+__device__ __forceinline__ int low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
+                                      0x05040100u);
+}
 
-// Activations (ACFUN_RELU and the others of the header).  exp by the hardware's 2^x: one
+// The largest over a wave's lanes, in every lane.
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+    v = umax(v, lane_perm<kXor1>(v));
+    v = umax(v, lane_perm<kXor2>(v));
+    v = umax(v, lane_perm<kMirror8>(v));
+    v = umax(v, lane_perm<kMirror16>(v));
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = umax(p[0], p[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return umax(q[0], q[1]);
+}
+// max|x| of eight values as bits of fp32, by the type's own bits (whose order without
+// sign is the values').
+__device__ __forceinline__ unsigned abs_max8(const f8u& v) {
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = umax(m, bits_abs(v[e]));
+    return m;
+}
+__device__ __forceinline__ unsigned abs_max8_16(const u4v& v) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    auto abs2 = [](unsigned u) { return as_pair<us2>(u & 0x7fff7fffu); };
+    const us2 m = __builtin_elementwise_max(__builtin_elementwise_max(abs2(v[0]), abs2(v[1])),
+                                            __builtin_elementwise_max(abs2(v[2]), abs2(v[3])));
+    return umax(m[0], m[1]);
+}
+__device__ __forceinline__ unsigned abs_max8(const b8u& v) { return abs_max8_16(__builtin_bit_cast(u4v, v)) << 16; }
+__device__ __forceinline__ unsigned abs_max8(const h8u& v) {
+    return __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)abs_max8_16(__builtin_bit_cast(u4v, v))));
+}
+// Eight values of a tensor of E as floats; eight codes as bytes.
+template <class E>
+__device__ __forceinline__ void floats8(const typename VecOf<E, 8>::type& v, float (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)v[e];
+}
+__device__ __forceinline__ int2 bytes8(const unsigned (&c)[8]) {
+    return {low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7])};
+}
+
+// Activations, as in the header.  exp by the hardware's 2^x: one
 // step of its argument is |v| / 2^24 of the result, which bf16 and fp16 do not show;
 // EXACT (fp32 results) adds what the argument's rounding lost.  NaN stays NaN.
 template <bool EXACT>
@@ -50,13 +122,14 @@ __device__ __forceinline__ float exp_of(float v) {
     const float d = __builtin_fmaf(v, L, -t) + v * l;
     return __builtin_fabsf(v) < 88.f ? __builtin_fmaf(e, d * ln2, e) : e;                // (past it e may be infinite)
 }
+constexpr int ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4;
 template <bool EXACT>
 __device__ __forceinline__ float act_value(float v, int act) {
     if (act == 0) return v;
-    if (act == 1) return __builtin_elementwise_maximum(v, 0.f);
-    if (act == 3) return 0.5f * v * erfcf(v * -0x1.6a09e6p-1f);
+    if (act == ACT_RELU) return __builtin_elementwise_maximum(v, 0.f);
+    if (act == ACT_GELU) return 0.5f * v * erfcf(v * -0x1.6a09e6p-1f);
     float z = v;
-    if (act == 4) z = 0x1.988454p+0f * (v + 0.044715f * v * v * v);                // 2 sqrt(2 / pi)
+    if (act == ACT_GELU_TANH) z = 0x1.988454p+0f * (v + 0.044715f * v * v * v);                // 2 sqrt(2 / pi)
     const float e = 1.f + exp_of<EXACT>(-z);
     if constexpr (EXACT) return v / e;
     return v * __builtin_amdgcn_rcpf(e);
