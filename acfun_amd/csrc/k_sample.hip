@@ -20,7 +20,6 @@ namespace acfun {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kThreads = kSampleThreads, kWaves = kThreads / 64, kBins = 2048, kList = 2048;
 
 // The order of the values as one of integers, equal for +0 and -0; 0 for those that are
 // never drawn, NaN and -infinity.
@@ -53,6 +52,16 @@ __device__ __forceinline__ double exp2_of(double t) {
 struct Weights {
     double max, c, one, least;                  // c: log2(e) / T; one: 2^f; least: min_p
     float top, per_2x;                          // the largest value; bins to two units of x
+    int bins;
+    // `bins` for the 50 powers of two that weigh; no infinity, whose product with 0 is none
+    __device__ __forceinline__ Weights(float largest, float T, float m, int frac, int n) {
+        max = top = largest;
+        c = 0x1.71547652b82fep+0 / (double)T;
+        one = (double)(1ull << frac);
+        least = m > 0.f ? m < 1.f ? m : 1. : 0.;
+        per_2x = __builtin_fminf((float)n * (float)(0x1.715476p+0 / 25.) / T, 1e30f);
+        bins = n;
+    }
     // log2 of the weight; past any float's range where there is none
     __device__ __forceinline__ double log(float x) const {
         const double t = x == top ? 0. : ((double)x - max) * c;
@@ -76,17 +85,20 @@ struct Weights {
         const double w = t > -50. ? exp2_of(t) : 0.;
         return w >= least ? fixed(w) : 0;
     }
-    // from 0 for the largest value up; kBins: no weight (so for a NaN or -infinity)
+    // from 0 for the largest value up; `bins`: no weight (so for a NaN or -infinity)
     __device__ __forceinline__ unsigned bin(float x) const {
         const float b = x == top ? 0.f : __builtin_fmaf(x, -0.5f, 0.5f * top) * per_2x;  // (top - x may pass fp32)
-        return b < (float)kBins ? (unsigned)b : kBins;
+        return b < (float)bins ? (unsigned)b : (unsigned)bins;
     }
 };
 
+// A workgroup's: two bins and two entries of the list to a thread.
+template <int NT>
 struct Shared {
+    static constexpr int kWaves = NT / 64, kBins = 2 * NT, kList = 2 * NT;
     u64 mass[kBins];
     u64 list[kList];
-    u64 part[kWaves + 1];
+    u64 part[kWaves];
     unsigned count[kBins];
     unsigned n, bin;
     u64 above;
@@ -102,14 +114,15 @@ __device__ __forceinline__ V wave_all(V v, F f) {
     for (int d = 1; d < 64; d *= 2) v = f(v, (V)__shfl_xor(v, d));
     return v;
 }
-template <class V, class F>
-__device__ __forceinline__ V block_all(V v, Shared& sm, F f) {
+template <int NT, class V, class F>
+__device__ __forceinline__ V block_all(V v, Shared<NT>& sm, F f) {
+    typedef std::conditional_t<sizeof(V) == 8, u64, unsigned> U;
     v = wave_all(v, f);
-    if ((threadIdx.x & 63) == 0) sm.part[threadIdx.x >> 6] = __builtin_bit_cast(std::conditional_t<sizeof(V) == 8, u64, unsigned>, v);
+    if ((threadIdx.x & 63) == 0) sm.part[threadIdx.x >> 6] = __builtin_bit_cast(U, v);
     __syncthreads();
-    auto get = [&](int i) { return __builtin_bit_cast(V, (std::conditional_t<sizeof(V) == 8, u64, unsigned>)sm.part[i]); };
-    v = get(0);
-    for (int i = 1; i < kWaves; ++i) v = f(v, get(i));
+    v = __builtin_bit_cast(V, (U)sm.part[threadIdx.x % (NT / 64)]);
+#pragma unroll
+    for (int d = 1; d < NT / 64; d *= 2) v = f(v, (V)__shfl_xor(v, d));
     __syncthreads();
     return v;
 }
@@ -122,18 +135,18 @@ __device__ __forceinline__ u64 wave_upto(u64 v) {
     }
     return v;
 }
-__device__ __forceinline__ u64 block_upto(u64 v, Shared& sm, u64& total) {
+template <int NT>
+__device__ __forceinline__ u64 block_upto(u64 v, Shared<NT>& sm, u64& total) {
+    constexpr int W = NT / 64;
     v = wave_upto(v);
     if ((threadIdx.x & 63) == 63) sm.part[threadIdx.x >> 6] = v;
     __syncthreads();
-    total = 0;
-    for (int i = 0; i < kWaves; ++i) {
-        const u64 o = sm.part[i];
-        if (i < (int)(threadIdx.x >> 6)) v += o;
-        total += o;
-    }
+    const u64 waves = wave_upto((int)(threadIdx.x & 63) < W ? sm.part[threadIdx.x % W] : 0);
+    total = __shfl(waves, W - 1);
+    const int w = threadIdx.x >> 6;
+    const u64 before = __shfl(waves, w ? w - 1 : 0);
     __syncthreads();
-    return v;
+    return w ? v + before : v;
 }
 
 // A row's values, 16 bytes of them to a lane, to f(x, index).
@@ -141,42 +154,48 @@ template <class T>
 struct Row {
     static constexpr int V = 16 / (int)sizeof(T);
     typedef typename VecOf<T, V>::type VT;
+    struct Some {
+        VT v;
+        int i;                                  // the first one's index
+    };
     const T* x;
     int cols;
-    // a lane's V values from index i
-    __device__ __forceinline__ VT load(int i) const { return load_vec<T, V>(x + i, cols - i, -__builtin_inff()); }
-    // from i0 to i1, both whole 64 V but for the row's end, by lanes of `threads`, U loads at once
-    template <int U, class F>
+    // V values from index i; at the row's end its last V, those before i as -infinity
+    __device__ __forceinline__ Some load(int i) const {
+        if (i + V <= cols) return {*(const VT*)(x + i), i};
+        if (cols < V) return {load_vec<T, V>(x + i, cols - i, -__builtin_inff()), i};
+        Some s{*(const VT*)(x + cols - V), cols - V};
+#pragma unroll
+        for (int e = 0; e < V; ++e) s.v[e] = s.i + e < i ? (T)-__builtin_inff() : s.v[e];
+        return s;
+    }
+    // from i0 to i1, apart by whole 64 V or at the row's end, by lanes t of `threads`.  (One copy
+    // of f: what runs a few times is fetched as it runs.)
+    template <class F>
     __device__ __forceinline__ void each(int i0, int i1, int t, int threads, F f) const {
         int i = i0 + t * V;
         const int step = threads * V;
-        for (; i + (U - 1) * step + V <= i1; i += U * step) {
-            VT v[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = *(const VT*)(x + i + u * step);
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < V; ++e) f((float)v[u][e], i + u * step + e);
-        }
+        if (i >= i1) return;
+        Some s = load(i);
 #pragma unroll 1
-        for (; i < i1; i += step) {
-            const VT v = load(i);
+        for (;; i += step) {
+            const Some c = s;
+            const bool more = i + step < i1;
+            if (more) s = load(i + step);
 #pragma unroll
-            for (int e = 0; e < V; ++e) f((float)v[e], i + e);
+            for (int e = 0; e < V; ++e) f((float)c.v[e], c.i + e);
+            if (!more) return;
         }
     }
-    template <int U, class F>
-    __device__ __forceinline__ void all(F f) const { each<U>(0, cols, threadIdx.x, kThreads, f); }
 };
 
 // The first bin up to and with which the bins hold `need` (at least 1); those before it
 // hold sm.above.  False if all of them hold less.
-template <class V>
-__device__ __forceinline__ bool find_bin(const V* bins, u64 need, Shared& sm) {
+template <int NT, class V>
+__device__ __forceinline__ bool find_bin(const V* bins, u64 need, Shared<NT>& sm) {
     const int t = threadIdx.x, b0 = 2 * t, b1 = b0 + 1;
     const u64 first = bins[b0], mine = first + bins[b1];
-    if (t == 0) sm.bin = kBins;
+    if (t == 0) sm.bin = 2 * NT;
     u64 total;
     const u64 above = block_upto(mine, sm, total) - mine;
     if (above < need && need <= above + mine) {
@@ -185,14 +204,15 @@ __device__ __forceinline__ bool find_bin(const V* bins, u64 need, Shared& sm) {
         sm.above = zero ? above : above + first;
     }
     __syncthreads();
-    return sm.bin < kBins;
+    return sm.bin < 2 * NT;
 }
 
 // The list's first n entries, the largest first; the rest of it up to a power of two is 0.
-__device__ void sort_list(u64* list, int n) {
+template <int NT>
+__device__ __forceinline__ void sort_list(u64* list, int n) {
     int size = 64;
     while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+    for (int i = n + threadIdx.x; i < size; i += NT) list[i] = 0;
     for (int run = 2; run <= size; run *= 2)
         for (int d = run / 2; d > 0; d /= 2) {
             __syncthreads();
@@ -205,47 +225,49 @@ __device__ void sort_list(u64* list, int n) {
     __syncthreads();
 }
 
-template <class T>
+template <class T, int NT>
 struct Draw {
+    static constexpr int kWaves = NT / 64, kBins = 2 * NT, kList = 2 * NT;
     const Row<T> row;
-    Weights w;
-    Shared& sm;
+    const Weights w;
+    Shared<NT>& sm;
+    int* const token;
+    float* const prob;
+    const float u;
 
-    // Tokens of the bins b0 to b1 into the list, in order; false if they are more than it holds.
-    __device__ bool gather(unsigned b0, unsigned b1) {
+    template <class F>
+    __device__ __forceinline__ void all(F f) const { row.each(0, row.cols, threadIdx.x, NT, f); }
+    __device__ __forceinline__ void clear() const {
+        sm.mass[threadIdx.x] = sm.mass[threadIdx.x + NT] = 0;
+        sm.count[threadIdx.x] = sm.count[threadIdx.x + NT] = 0;
         if (threadIdx.x == 0) sm.n = 0;
         __syncthreads();
-        row.template all<4>([&](float x, int i) {
+    }
+    // Tokens i0 to i1 of the bins b0 to b1 to take(n, place), n counting them.
+    template <class F>
+    __device__ __forceinline__ void gather(int i0, int i1, unsigned b0, unsigned b1, unsigned* n, F take) const {
+        row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) {
             const unsigned b = w.bin(x);
-            if (b < b0 || b > b1) return;
-            const unsigned at = atomicAdd(&sm.n, 1u);
-            if (at < kList) sm.list[at] = place_of(x, i);
+            if (b >= b0 && b <= b1) take(atomicAdd(n, 1u), place_of(x, i));
         });
-        __syncthreads();
-        const unsigned n = sm.n;
-        __syncthreads();
-        if (n > kList) return false;
-        sort_list(sm.list, (int)n);
-        return true;
     }
 
     // The cut in bin b: the first place of its tokens, in order, up to and with which their
-    // number or mass, `before` with what the earlier bins hold, is `need`; `upto` becomes the
-    // mass (MASS) up to and with it.  For bins of any size: by its digits, a pass for each.
+    // number or mass, `before` with what the earlier bins hold, is `need`.  For bins of
+    // any size: by its digits, a pass for each.
     template <bool MASS>
-    __device__ u64 cut_by_digits(unsigned b, u64 need, u64 before) {
+    __device__ __forceinline__ u64 cut_by_digits(unsigned b, u64 need, u64 before) const {
         u64 prefix = 0;
-        for (int shift = 53;; shift = shift > 11 ? shift - 11 : 0) {
-            const int width = shift ? 11 : 9;
-            for (int i = threadIdx.x; i < kBins; i += kThreads) {
-                if constexpr (MASS) sm.mass[i] = 0;
-                else sm.count[i] = 0;
-            }
-            __syncthreads();
-            row.template all<1>([&](float x, int i) {
+        constexpr int D = NT == 1024 ? 11 : 9;
+        static_assert(1 << D <= kBins, "a bin to each digit");
+#pragma unroll 1
+        for (int shift = 64 - D;;) {
+            const int width = shift == 0 ? (64 - 1) % D + 1 : D;
+            clear();
+            all([&](float x, int i) {
                 if (w.bin(x) != b) return;
                 const u64 p = place_of(x, i);
-                if (shift < 53 && p >> (shift + width) != prefix) return;
+                if (shift < 64 - D && p >> (shift + width) != prefix) return;
                 const unsigned d = (1u << width) - 1 - ((unsigned)(p >> shift) & ((1u << width) - 1));   // the largest first
                 if constexpr (MASS) atomicAdd(&sm.mass[d], w(x));
                 else atomicAdd(&sm.count[d], 1u);
@@ -257,98 +279,111 @@ struct Draw {
             before += sm.above;
             __syncthreads();
             if (shift == 0) return prefix;
+            shift = shift > D ? shift - D : 0;
         }
     }
-    template <bool MASS>
-    __device__ u64 cut(unsigned b, u64 need, u64 before) {
-        if (!gather(b, b)) return cut_by_digits<MASS>(b, need, before);
-        u64 total;
-        const int t = threadIdx.x, n = (int)sm.n;
-        const u64 p0 = 2 * t < n ? sm.list[2 * t] : 0, p1 = 2 * t + 1 < n ? sm.list[2 * t + 1] : 0;
-        u64 m0, m1;
-        if constexpr (MASS) m0 = p0 ? w(value_of(p0 >> 32)) : 0, m1 = p1 ? w(value_of(p1 >> 32)) : 0;
-        else m0 = p0 != 0, m1 = p1 != 0;
-        const u64 upto = before + block_upto(m0 + m1, sm, total), first = upto - m1;
-        if (first - m0 < need && need <= upto) sm.above = first >= need ? p0 : p1;
-        __syncthreads();
-        const u64 c = sm.above;
-        __syncthreads();
-        return c;
-    }
-
-    // Draws from the first n of the list, which is in order, with u; the total's weight.
-    __device__ void from_list(int n, float u, int* token, float* prob) {
+    // The same of a bin whose tokens are the list's n, in order.
+    __device__ __forceinline__ u64 cut_in_list(int n, bool mass, u64 need, u64 before) const {
         const int t = threadIdx.x;
         u64 p[2], m[2], total;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             p[e] = 2 * t + e < n ? sm.list[2 * t + e] : 0;
-            p[e] = p[e] << 32 | p[e] >> 32;     // by index: ~i is the larger half
+            m[e] = !p[e] ? 0 : mass ? w(value_of(p[e] >> 32)) : 1;
         }
+        const u64 upto = before + block_upto(m[0] + m[1], sm, total), first = upto - m[1];
+        if (first - m[0] < need && need <= upto) sm.above = first >= need ? p[0] : p[1];
         __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (2 * t + e < n) sm.list[2 * t + e] = p[e];
+        const u64 c = sm.above;
         __syncthreads();
-        sort_list(sm.list, n);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            p[e] = 2 * t + e < n ? sm.list[2 * t + e] : 0;
-            m[e] = p[e] ? w.kept(value_of((unsigned)p[e])) : 0;
-        }
-        const u64 upto = block_upto(m[0] + m[1], sm, total), before = upto - m[0] - m[1];
-        const u64 target = target_of(u, total);
-        if (target == 0 && u64_zero(u, n, token, prob, total)) return;
-        if (before <= target && target < upto) {
-            const bool one = target >= before + m[0];
-            put(~(int)(p[one] >> 32), value_of((unsigned)p[one]), total, token, prob);
-        }
+        return c;
     }
-    __device__ __forceinline__ u64 target_of(float u, u64 total) const {
+    // The part p of a mass, in steps, at least one.
+    __device__ __forceinline__ u64 share(float p, u64 of) const {
+        const double want = __builtin_ceil((double)p * (double)of);
+        return want >= 1. ? (u64)want : 1;
+    }
+    __device__ __forceinline__ u64 target_of(u64 total) const {
         const double at = (double)(u > 0.f ? u < 1.f ? u : 0x1.fffffep-1f : 0.f) * (double)total;
         return (u64)at < total ? (u64)at : total - 1;
     }
-    __device__ __forceinline__ void put(int i, float x, u64 total, int* token, float* prob) const {
+    __device__ __forceinline__ void put(int i, float x, u64 total) const {
         *token = i;
         if (prob) *prob = (float)(w.real(x) * w.one / (double)total);
     }
-    // u = 0 among the list: the first kept, however small its weight
-    __device__ bool u64_zero(float, int n, int* token, float* prob, u64 total) {
+
+    // Draws from the list's n tokens, all those of the first bins: of the first k (0: all), of
+    // these the first that reach p of their mass, or of `all` (0: theirs).
+    __device__ __forceinline__ void from_list(int n, int k, float p, u64 all) const {
         const int t = threadIdx.x;
-        int first = kList;
-        for (int j = 2 * t + 1; j >= 2 * t; --j)
-            if (j < n) {
-                const double v = w.real(value_of((unsigned)sm.list[j]));
-                if (v > 0. && v >= w.least) first = j;
+        sort_list<NT>(sm.list, n);
+        if (k && n > k) n = k;
+        u64 q[2], m[2], total;
+#pragma unroll 1
+        for (int pass = 0;; ++pass) {           // first in order, then by index
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                q[e] = 2 * t + e < n ? sm.list[2 * t + e] : 0;
+                m[e] = q[e] ? (pass ? w.kept(value_of((unsigned)q[e])) : w(value_of(q[e] >> 32))) : 0;
+            }
+            const u64 upto = block_upto(m[0] + m[1], sm, total), first = upto - m[1], before = first - m[0];
+            if (pass) {
+                const u64 target = target_of(total);
+                if (target == 0) break;
+                if (before <= target && target < upto) {
+                    const u64 at = target >= first ? q[1] : q[0];
+                    put(~(int)(at >> 32), value_of((unsigned)at), total);
+                }
+                return;
+            }
+            if (p < 1.f) {                      // a token is kept while those before it stay below the share
+                const u64 need = share(p, all ? all : total);
+                n = block_all((2 * t < n && before < need) + (2 * t + 1 < n && first < need), sm, Add{});
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (2 * t + e < n) sm.list[2 * t + e] = q[e] << 32 | q[e] >> 32;
+            __syncthreads();
+            sort_list<NT>(sm.list, n);
+        }
+        int first = kList;                      // u = 0: the first kept, however small its weight
+#pragma unroll
+        for (int e = 1; e >= 0; --e)
+            if (2 * t + e < n) {
+                const double v = w.real(value_of((unsigned)q[e]));
+                if (v > 0. && v >= w.least) first = 2 * t + e;
             }
         first = block_all(first, sm, Min{});
-        if (t == 0) put(~(int)(sm.list[first] >> 32), value_of((unsigned)sm.list[first]), total, token, prob);
-        return true;
+        if (t == 0) put(~(int)(sm.list[first] >> 32), value_of((unsigned)sm.list[first]), total);
     }
 
-    // Draws from all tokens of the row not below the cut.
-    __device__ void from_row(u64 cut, float u, int* token, float* prob) {
+    // The mass of the tokens a to b not below the cut, in every lane of a wave.
+    __device__ __forceinline__ u64 kept_mass(int a, int b, u64 cut, int t, int threads) const {
+        u64 mass = 0;
+        row.each(a, b, t, threads, [&](float x, int i) {
+            if (i < b && place_of(x, i) >= cut) mass += w.kept(x);
+        });
+        return wave_all(mass, Add{});
+    }
+    // Draws from the tokens i0 to i1 not below the cut, those before them having the mass
+    // `before` of all tokens' `total` (known: false if i0 to i1 are all tokens).
+    __device__ __forceinline__ void from_row(int i0, int i1, u64 cut, bool known, u64 before, u64 total) const {
         constexpr int Q = 64 * Row<T>::V;       // a wave's values at once
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        auto kept = [&](float x, int i) { return place_of(x, i) >= cut ? w.kept(x) : 0; };
-        // a run of the row to each wave, then a part of the run that it falls in
-        int i0 = 0, i1 = row.cols;
-        u64 before = 0, total = 0, target = 0;
-        for (int level = 0;; ++level) {
+        u64 target = known ? target_of(total) : 1;
+        // a run to each wave, then a part of the run that the target falls in
+#pragma unroll 1
+        while (target) {
             const int per = ((i1 - i0 + kWaves - 1) / kWaves + Q - 1) / Q * Q;
             const int a = i0 + wave * per < i1 ? i0 + wave * per : i1, b = a + per < i1 ? a + per : i1;
-            u64 mass = 0;
-            row.template each<2>(a, b, lane, 64, [&](float x, int i) { mass += i < b ? kept(x, i) : 0; });
-            mass = wave_all(mass, Add{});
+            const u64 mass = kept_mass(a, b, cut, lane, 64);
             if (lane == 0) sm.part[wave] = mass;
             __syncthreads();
-            if (level == 0) {
-                for (int i = 0; i < kWaves; ++i) total += sm.part[i];
-                target = target_of(u, total);
-                if (target == 0) break;
-            }
-            int s = 0;
-            for (; s < kWaves - 1 && target >= before + sm.part[s]; ++s) before += sm.part[s];
+            const u64 upto = wave_upto(lane < kWaves ? sm.part[lane % kWaves] : 0);
+            if (!known) total = __shfl(upto, kWaves - 1), target = target_of(total), known = true;
+            const u64 past = __ballot(lane < kWaves && before + upto > target);
+            const int s = past ? __ffsll(past) - 1 : kWaves - 1;
+            before += s ? __shfl(upto, s - 1) : 0;
             __syncthreads();
             i0 += s * per;
             i1 = i0 + per < i1 ? i0 + per : i1;
@@ -356,155 +391,152 @@ struct Draw {
         }
         if (target == 0) {                      // u = 0: the first kept, however small its weight
             int first = row.cols;
-            row.template all<1>([&](float x, int i) {
+            all([&](float x, int i) {
                 if (i >= first || place_of(x, i) < cut) return;
                 const double v = w.real(x);
                 if (v > 0. && v >= w.least) first = i;
             });
             __syncthreads();
             first = block_all(first, sm, Min{});
-            if (threadIdx.x == 0) put(first, (float)row.x[first], total, token, prob);
+            if (threadIdx.x == 0) put(first, (float)row.x[first], total);
             return;
         }
         if (wave) return;
-        const auto v = row.load(i0 + lane * Row<T>::V);
-        u64 mine = 0;
+        const auto v = row.load(i0 + lane * Row<T>::V < row.cols ? i0 + lane * Row<T>::V : row.cols);
+        u64 m[Row<T>::V], mine = 0;
 #pragma unroll
-        for (int e = 0; e < Row<T>::V; ++e) mine += kept((float)v[e], i0 + lane * Row<T>::V + e);
+        for (int e = 0; e < Row<T>::V; ++e) {
+            m[e] = v.i + e < i1 && place_of((float)v.v[e], v.i + e) >= cut ? w.kept((float)v.v[e]) : 0;
+            mine += m[e];
+        }
         before += wave_upto(mine) - mine;
         if (target < before || target >= before + mine) return;
+        int at = 0;
+        float x = 0.f;
+#pragma unroll
         for (int e = 0; e < Row<T>::V; ++e) {
-            const int i = i0 + lane * Row<T>::V + e;
-            const float x = (float)row.x[i];
-            before += kept(x, i);
-            if (before > target) {
-                put(i, x, total, token, prob);
+            if (before <= target && target < before + m[e]) at = v.i + e, x = (float)v.v[e];
+            before += m[e];
+        }
+        put(at, x, total);
+    }
+
+    // A whole row, whose largest value is w.top, with its first k and p (1 or more: all).
+    __device__ __forceinline__ void from_whole(int k, float p) const {
+        const int t = threadIdx.x;
+        const bool nucleus = p < 1.f;
+        u64 cut = 1ull << 32;                   // all that can be drawn
+        if (k > 0 || nucleus) {
+            clear();
+            all([&](float x, int) {
+                const unsigned b = w.bin(x);
+                if (b >= (unsigned)kBins) return;
+                atomicAdd(&sm.count[b], 1u);
+                if (nucleus) atomicAdd(&sm.mass[b], w(x));
+            });
+            __syncthreads();
+        }
+        u64 mass = 0;
+        bool first = true;
+#pragma unroll 1
+        for (bool by_count = k > 0;; by_count = false, first = false) {
+            if (!by_count && !nucleus) break;
+            u64 need = (u64)k;
+            if (by_count) {                     // (fewer tokens than k that weigh anything: no limit)
+                if (!find_bin(sm.count, need, sm)) {
+                    k = 0, by_count = false;
+                    __syncthreads();
+                    if (!nucleus) break;
+                }
+            }
+            if (!by_count) {
+                mass = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{});
+                need = share(p, mass);
+                find_bin(sm.mass, need, sm);
+            }
+            const unsigned b = sm.bin;
+            const u64 above = sm.above;
+            // how many the bins up to b hold: few are all taken
+            unsigned few = (2 * t <= (int)b ? sm.count[2 * t] : 0) + (2 * t + 1 <= (int)b ? sm.count[2 * t + 1] : 0);
+            few = block_all(few, sm, Add{});
+            const bool take = first && few <= (unsigned)kList;
+            if (t == 0) sm.n = 0;
+            __syncthreads();
+            gather(0, row.cols, take ? 0 : b, b, &sm.n, [&](unsigned at, u64 place) {
+                if (at < (unsigned)kList) sm.list[at] = place;
+            });
+            __syncthreads();
+            const int n = (int)sm.n;
+            if (take) {
+                from_list(n, k, p, by_count ? 0 : mass);
                 return;
             }
+            __syncthreads();
+            if (n <= kList) {
+                sort_list<NT>(sm.list, n);
+                cut = cut_in_list(n, !by_count, need, above);
+            } else {
+                cut = by_count ? cut_by_digits<false>(b, need, above) : cut_by_digits<true>(b, need, above);
+            }
+            if (!by_count || !nucleus) break;
+            clear();                            // the mass of the tokens up to the cut
+            all([&](float x, int i) {
+                const unsigned b = w.bin(x);
+                if (b < (unsigned)kBins && place_of(x, i) >= cut) atomicAdd(&sm.mass[b], w(x));
+            });
+            __syncthreads();
         }
+        from_row(0, row.cols, cut, false, 0, 0);
     }
 };
 
-template <class T>
-__global__ __launch_bounds__(kThreads) void k_sample(SampleArgs a, int frac) {
-    __shared__ Shared sm;
-    const int t = threadIdx.x, r = blockIdx.x;
-    Draw<T> d{{(const T*)a.x + (size_t)r * a.ld, a.cols}, {}, sm};
-    int* const token = a.token + r;
-    float* const prob = a.prob ? a.prob + r : nullptr;
+// A row's largest value with its lowest index, as its place; 0 for a row with nothing to draw.
+template <int NT, class T>
+__device__ __forceinline__ u64 first_of(const Row<T>& row, int i0, int i1, Shared<NT>& sm) {
     float top = -__builtin_inff();
-    d.row.template all<4>([&](float x, int) { top = __builtin_fmaxf(top, x); });
-    top = block_all(top, sm, [](float p, float q) { return __builtin_fmaxf(p, q); });
-    if (top == -__builtin_inff()) {
-        if (t == 0) {
-            *token = -1;
-            if (prob) *prob = 0.f;
-        }
-        return;
+    int at = 0;
+    row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) {
+        const bool more = x > top && i < i1;
+        top = more ? x : top;
+        at = more ? i : at;
+    });
+    return block_all(top > -__builtin_inff() ? place_of(top, at) : 0, sm, Max{});
+}
+// What a row asks for.
+struct Ask {
+    float T, p, m, u;
+    int k;
+    __device__ __forceinline__ Ask(const SampleArgs& a, int r) {
+        T = a.temp ? a.temp[r] : 1.f;
+        p = a.top_p ? a.top_p[r] : 1.f;
+        m = a.min_p ? a.min_p[r] : 0.f;
+        u = a.u[r];
+        k = a.top_k ? a.top_k[r] : 0;
+        if (k < 0 || k >= a.cols) k = 0;
     }
-    const float T0 = a.temp ? a.temp[r] : 1.f, m = a.min_p ? a.min_p[r] : 0.f, u = a.u[r];
-    if (!(T0 > 0.f)) {
-        int first = a.cols;
-        d.row.template all<4>([&](float x, int i) { first = x == top && i < first ? i : first; });
-        first = block_all(first, sm, Min{});
-        if (t == 0) {
-            *token = first;
-            if (prob) *prob = 1.f;
-        }
-        return;
+};
+// A row that needs no draw: nothing in it, or the largest asked for.
+__device__ __forceinline__ bool settled(const SampleArgs& a, int r, u64 first, const Ask& ask) {
+    if (first && ask.T > 0.f) return false;
+    if (threadIdx.x == 0) {
+        a.token[r] = first ? ~(int)first : -1;
+        if (a.prob) a.prob[r] = first ? 1.f : 0.f;
     }
-    Weights& w = d.w;
-    w.max = top;
-    w.c = 0x1.71547652b82fep+0 / (double)T0;
-    w.one = (double)(1ull << frac);
-    w.least = m > 0.f ? m < 1.f ? m : 1. : 0.;
-    w.top = top;
-    // kBins for the 50 powers of two that weigh; no infinity, whose product with 0 is none
-    w.per_2x = __builtin_fminf((float)(kBins / 25.) * (0x1.715476p+0f / T0), 1e30f);
-    int k = a.top_k ? a.top_k[r] : 0;
-    float p = a.top_p ? a.top_p[r] : 1.f;
-    const bool nucleus = p < 1.f;
-    u64 cut = 1ull << 32;                       // all that can be drawn
-    if (k <= 0 || k >= a.cols) k = 0;
-    if (k || nucleus) {
-        for (int i = t; i < kBins; i += kThreads) sm.mass[i] = 0, sm.count[i] = 0;
-        __syncthreads();
-        d.row.template all<2>([&](float x, int) {
-            const unsigned b = w.bin(x);
-            if (b >= kBins) return;
-            atomicAdd(&sm.count[b], 1u);
-            if (nucleus) atomicAdd(&sm.mass[b], w(x));
-        });
-        __syncthreads();
-        // (fewer tokens than k that weigh anything: no limit)
-        if (k && !find_bin(sm.count, (u64)k, sm)) k = 0;
-        unsigned b = sm.bin;
-        u64 above = sm.above, all = 0, need = 0;
-        __syncthreads();
-        if (!k && !nucleus) {
-            d.from_row(cut, u, token, prob);
-            return;
-        }
-        if (nucleus) {
-            u64 mine = sm.mass[2 * t] + sm.mass[2 * t + 1];
-            all = block_all(mine, sm, Add{});
-        }
-        auto share = [&](u64 of) {
-            const double want = __builtin_ceil((double)p * (double)of);
-            return want >= 1. ? (u64)want : 1;
-        };
-        if (!k) {
-            need = share(all);
-            find_bin(sm.mass, need, sm);
-            b = sm.bin;
-            above = sm.above;
-            __syncthreads();
-        }
-        // how many the bins up to b hold
-        u64 few = 0;
-        for (int i = 2 * t; i < 2 * t + 2; ++i) few += i <= (int)b ? sm.count[i] : 0;
-        few = block_all(few, sm, Add{});
-        if (few <= kList) {
-            d.gather(0, b);
-            int n = (int)sm.n;
-            if (k && n > k) n = k;
-            if (nucleus) {
-                u64 mass[2], total;
-                for (int e = 0; e < 2; ++e) mass[e] = 2 * t + e < n ? w(value_of(sm.list[2 * t + e] >> 32)) : 0;
-                const u64 upto = block_upto(mass[0] + mass[1], sm, total);
-                if (k) need = share(total);
-                // a token is kept while those before it stay below `need`
-                const u64 b1 = upto - mass[1], b0 = b1 - mass[0];
-                u64 mine = (2 * t < n && b0 < need) + (2 * t + 1 < n && b1 < need);
-                n = (int)block_all(mine, sm, Add{});
-            }
-            d.from_list(n, u, token, prob);
-            return;
-        }
-        if (k) {
-            cut = d.template cut<false>(b, (u64)k, above);
-            if (nucleus) {
-                // of the tokens up to the cut: their mass, and the bin that holds p of it
-                for (int i = t; i < kBins; i += kThreads) sm.mass[i] = 0;
-                __syncthreads();
-                d.row.template all<2>([&](float x, int i) {
-                    const unsigned b = w.bin(x);
-                    if (b < kBins && place_of(x, i) >= cut) atomicAdd(&sm.mass[b], w(x));
-                });
-                __syncthreads();
-                all = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{});
-                need = share(all);
-                find_bin(sm.mass, need, sm);
-                b = sm.bin;
-                above = sm.above;
-                __syncthreads();
-                cut = d.template cut<true>(b, need, above);
-            }
-        } else {
-            cut = d.template cut<true>(b, need, above);
-        }
-    }
-    d.from_row(cut, u, token, prob);
+    return true;
+}
+
+// A workgroup to a row, which it reads three to five times.
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void k_sample(SampleArgs a, int frac) {
+    __shared__ Shared<NT> sm;
+    const int r = blockIdx.x;
+    const Row<T> row{(const T*)a.x + (size_t)r * a.ld, a.cols};
+    const Ask ask(a, r);
+    const u64 first = first_of(row, 0, a.cols, sm);
+    if (settled(a, r, first, ask)) return;
+    const Draw<T, NT> d{row, Weights(value_of(first >> 32), ask.T, ask.m, frac, 2 * NT), sm, a.token + r,
+                        a.prob ? a.prob + r : nullptr, ask.u};
+    d.from_whole(ask.k, ask.p);
 }
 
 }  // namespace
@@ -512,9 +544,13 @@ __global__ __launch_bounds__(kThreads) void k_sample(SampleArgs a, int frac) {
 bool sample_rows(const SampleArgs& a, int type, hipStream_t s) {
     int bits = 0;
     while ((1 << bits) < a.cols) ++bits;
+    const int frac = 62 - bits < 48 ? 62 - bits : 48;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        ACFUN_LAUNCH("k_sample", k_sample<T>, dim3(a.rows), dim3(kThreads), 0, s, a, 62 - bits < 48 ? 62 - bits : 48);
+        if (a.cols <= kSampleShort)
+            ACFUN_LAUNCH("k_sample", (k_sample<T, 256>), dim3(a.rows), dim3(256), 0, s, a, frac);
+        else
+            ACFUN_LAUNCH("k_sample", (k_sample<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a, frac);
         return check_launch("k_sample");
     });
 }
