@@ -243,15 +243,6 @@ struct Draw {
         if (threadIdx.x == 0) sm.n = 0;
         __syncthreads();
     }
-    // Tokens i0 to i1 of the bins b0 to b1 to take(n, place), n counting them.
-    template <class F>
-    __device__ __forceinline__ void gather(int i0, int i1, unsigned b0, unsigned b1, unsigned* n, F take) const {
-        row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) {
-            const unsigned b = w.bin(x);
-            if (b >= b0 && b <= b1) take(atomicAdd(n, 1u), place_of(x, i));
-        });
-    }
-
     // The cut in bin b: the first place of its tokens, in order, up to and with which their
     // number or mass, `before` with what the earlier bins hold, is `need`.  For bins of
     // any size: by its digits, a pass for each.
@@ -421,70 +412,90 @@ struct Draw {
         put(at, x, total);
     }
 
-    // A whole row, whose largest value is w.top, with its first k and p (1 or more: all).
-    __device__ __forceinline__ void from_whole(int k, float p) const {
+    // What the histogram says of the row's first k (0: all) and p (1 or more: all): the bin
+    // that the next cut lies in, and whether the tokens up to it are few enough to take them all.
+    struct Plan {
+        bool by_count, cut, take;               // cut: there is one
+        int k;
+        unsigned bin;
+        u64 need, above, mass;                  // mass: of all tokens (not by_count)
+    };
+    __device__ __forceinline__ Plan plan(int k, float p, bool by_count) const {
         const int t = threadIdx.x;
-        const bool nucleus = p < 1.f;
-        u64 cut = 1ull << 32;                   // all that can be drawn
-        if (k > 0 || nucleus) {
-            clear();
-            all([&](float x, int) {
-                const unsigned b = w.bin(x);
-                if (b >= (unsigned)kBins) return;
-                atomicAdd(&sm.count[b], 1u);
-                if (nucleus) atomicAdd(&sm.mass[b], w(x));
-            });
+        Plan l{by_count, true, false, k, 0, (u64)k, 0, 0};
+        if (by_count && !find_bin(sm.count, l.need, sm)) {      // fewer tokens than k that weigh anything: no limit
+            l.k = 0, l.by_count = false;
             __syncthreads();
         }
-        u64 mass = 0;
-        bool first = true;
+        if (!l.by_count) {
+            if (!(p < 1.f)) {
+                l.cut = false;
+                return l;
+            }
+            l.mass = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{});
+            l.need = share(p, l.mass);
+            find_bin(sm.mass, l.need, sm);
+        }
+        l.bin = sm.bin;
+        l.above = sm.above;
+        const unsigned few =
+            (2 * t <= (int)l.bin ? sm.count[2 * t] : 0) + (2 * t + 1 <= (int)l.bin ? sm.count[2 * t + 1] : 0);
+        l.take = block_all(few, sm, Add{}) <= (unsigned)kList;
+        return l;
+    }
+    // The histogram of the tokens i0 to i1 not below the cut.
+    __device__ __forceinline__ void fill(int i0, int i1, bool count, bool mass, u64 cut) const {
+        row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) {
+            const unsigned b = w.bin(x);
+            if (b >= (unsigned)kBins || i >= i1 || (cut >> 32 && place_of(x, i) < cut)) return;
+            if (count) atomicAdd(&sm.count[b], 1u);
+            if (mass) atomicAdd(&sm.mass[b], w(x));
+        });
+        __syncthreads();
+    }
+    // Tokens i0 to i1 of the bins up to l's (l.take) or of that alone to the list; their number.
+    __device__ __forceinline__ unsigned gather(int i0, int i1, const Plan& l) const {
+        if (threadIdx.x == 0) sm.n = 0;
+        __syncthreads();
+        const unsigned b0 = l.take ? 0 : l.bin;
+        row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) {
+            const unsigned b = w.bin(x);
+            if (b < b0 || b > l.bin || i >= i1) return;
+            const unsigned at = atomicAdd(&sm.n, 1u);
+            if (at < (unsigned)kList) sm.list[at] = place_of(x, i);
+        });
+        __syncthreads();
+        const unsigned n = sm.n;
+        __syncthreads();
+        return n;
+    }
+    // The cut of l, from the list's n tokens of its bin (more than it holds: from the row).
+    __device__ __forceinline__ u64 cut_of(const Plan& l, unsigned n) const {
+        if (n > (unsigned)kList)
+            return l.by_count ? cut_by_digits<false>(l.bin, l.need, l.above) : cut_by_digits<true>(l.bin, l.need, l.above);
+        sort_list<NT>(sm.list, (int)n);
+        return cut_in_list((int)n, !l.by_count, l.need, l.above);
+    }
+
+    // A whole row, whose largest value is w.top.
+    __device__ __forceinline__ void from_whole(int k, float p) const {
+        u64 cut = 1ull << 32;                   // all that can be drawn
+        bool by_count = k > 0;
 #pragma unroll 1
-        for (bool by_count = k > 0;; by_count = false, first = false) {
-            if (!by_count && !nucleus) break;
-            u64 need = (u64)k;
-            if (by_count) {                     // (fewer tokens than k that weigh anything: no limit)
-                if (!find_bin(sm.count, need, sm)) {
-                    k = 0, by_count = false;
-                    __syncthreads();
-                    if (!nucleus) break;
-                }
-            }
-            if (!by_count) {
-                mass = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{});
-                need = share(p, mass);
-                find_bin(sm.mass, need, sm);
-            }
-            const unsigned b = sm.bin;
-            const u64 above = sm.above;
-            // how many the bins up to b hold: few are all taken
-            unsigned few = (2 * t <= (int)b ? sm.count[2 * t] : 0) + (2 * t + 1 <= (int)b ? sm.count[2 * t + 1] : 0);
-            few = block_all(few, sm, Add{});
-            const bool take = first && few <= (unsigned)kList;
-            if (t == 0) sm.n = 0;
-            __syncthreads();
-            gather(0, row.cols, take ? 0 : b, b, &sm.n, [&](unsigned at, u64 place) {
-                if (at < (unsigned)kList) sm.list[at] = place;
-            });
-            __syncthreads();
-            const int n = (int)sm.n;
-            if (take) {
-                from_list(n, k, p, by_count ? 0 : mass);
+        for (bool first = true; by_count || p < 1.f; first = false) {
+            clear();
+            fill(0, row.cols, first, p < 1.f, first ? 0 : cut);
+            Plan l = plan(k, p, by_count);
+            if (!l.cut) break;
+            l.take &= first;
+            const unsigned n = gather(0, row.cols, l);
+            if (l.take) {
+                from_list((int)n, l.k, p, l.mass);
                 return;
             }
-            __syncthreads();
-            if (n <= kList) {
-                sort_list<NT>(sm.list, n);
-                cut = cut_in_list(n, !by_count, need, above);
-            } else {
-                cut = by_count ? cut_by_digits<false>(b, need, above) : cut_by_digits<true>(b, need, above);
-            }
-            if (!by_count || !nucleus) break;
-            clear();                            // the mass of the tokens up to the cut
-            all([&](float x, int i) {
-                const unsigned b = w.bin(x);
-                if (b < (unsigned)kBins && place_of(x, i) >= cut) atomicAdd(&sm.mass[b], w(x));
-            });
-            __syncthreads();
+            cut = cut_of(l, n);
+            if (!l.by_count || !(p < 1.f)) break;
+            by_count = false;                   // p of the tokens up to the cut
         }
         from_row(0, row.cols, cut, false, 0, 0);
     }
@@ -539,14 +550,179 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a, int frac) {
     d.from_whole(ask.k, ask.p);
 }
 
+// ---------------------------------------------------------------- few long rows
+// A row's `parts` workgroups have `per` of its tokens each, in four launches: the largest,
+// the histogram, the list, the draw.
+struct Split {
+    SampleArgs a;
+    int frac, parts, per;
+    char* rows;
+};
+constexpr int NS = 1024;                        // threads
+struct SplitRow {
+    u64 mass[Shared<NS>::kBins], list[Shared<NS>::kList];
+    u64 first[kSampleParts], kept[kSampleParts];
+    unsigned count[Shared<NS>::kBins];
+    unsigned n, done;
+};
+template <class T>
+struct Part {
+    const int r, part, i0, i1;
+    const Row<T> row;
+    SplitRow& ws;
+    __device__ __forceinline__ explicit Part(const Split& p)
+        : r(blockIdx.y), part(blockIdx.x), i0(part * p.per), i1(i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols),
+          row{(const T*)p.a.x + (size_t)r * p.a.ld, p.a.cols}, ws(((SplitRow*)p.rows)[r]) {}
+    __device__ __forceinline__ u64 first(const Split& p) const {
+        const int lane = threadIdx.x & 63;
+        return wave_all(lane < p.parts ? ws.first[lane] : 0, Max{});
+    }
+    __device__ __forceinline__ Draw<T, NS> draw(const Split& p, u64 top, const Ask& ask, Shared<NS>& sm) const {
+        return {row, Weights(value_of(top >> 32), ask.T, ask.m, p.frac, 2 * NS), sm, p.a.token + r,
+                p.a.prob ? p.a.prob + r : nullptr, ask.u};
+    }
+};
+// Those that are settled without a histogram.
+__device__ __forceinline__ bool plain(u64 top, const Ask& ask) {
+    return !top || !(ask.T > 0.f) || (!ask.k && !(ask.p < 1.f));
+}
+
+template <class T>
+__global__ __launch_bounds__(NS) void k_sample_first(Split p) {
+    __shared__ Shared<NS> sm;
+    const Part<T> q(p);
+    for (int i = q.part * NS + threadIdx.x; i < 2 * NS; i += p.parts * NS) q.ws.mass[i] = 0, q.ws.count[i] = 0;
+    if (q.part == 0 && threadIdx.x == 0) q.ws.n = 0, q.ws.done = 0;
+    const u64 top = first_of(q.row, q.i0, q.i1, sm);
+    if (threadIdx.x == 0) q.ws.first[q.part] = top;
+}
+
+template <class T>
+__global__ __launch_bounds__(NS) void k_sample_bins(Split p) {
+    __shared__ Shared<NS> sm;
+    const Part<T> q(p);
+    const Ask ask(p.a, q.r);
+    const u64 top = q.first(p);
+    if (plain(top, ask)) return;
+    const auto d = q.draw(p, top, ask, sm);
+    d.clear();
+    d.fill(q.i0, q.i1, true, ask.p < 1.f, 0);
+#pragma unroll
+    for (int i = threadIdx.x; i < 2 * NS; i += NS) {
+        if (sm.count[i]) atomicAdd(&q.ws.count[i], sm.count[i]);
+        if (sm.mass[i]) atomicAdd(&q.ws.mass[i], sm.mass[i]);
+    }
+}
+
+// The row's histogram from memory, and its plan.
+template <class T>
+__device__ __forceinline__ typename Draw<T, NS>::Plan plan_of(const Part<T>& q, const Draw<T, NS>& d, const Ask& ask) {
+    for (int i = threadIdx.x; i < 2 * NS; i += NS) d.sm.count[i] = q.ws.count[i], d.sm.mass[i] = q.ws.mass[i];
+    __syncthreads();
+    return d.plan(ask.k, ask.p, ask.k > 0);
+}
+// A top-k of many tokens with a nucleus among them: one workgroup does such a row.
+template <class L>
+__device__ __forceinline__ bool hard(const L& l, const Ask& ask) { return l.by_count && !l.take && ask.p < 1.f; }
+
+template <class T>
+__global__ __launch_bounds__(NS) void k_sample_take(Split p) {
+    __shared__ Shared<NS> sm;
+    const Part<T> q(p);
+    const Ask ask(p.a, q.r);
+    const u64 top = q.first(p);
+    if (plain(top, ask)) return;
+    const auto d = q.draw(p, top, ask, sm);
+    const auto l = plan_of(q, d, ask);
+    if (!l.cut || hard(l, ask)) return;
+    const unsigned n = d.gather(q.i0, q.i1, l);
+    if (n == 0) return;
+    if (threadIdx.x == 0) sm.bin = atomicAdd(&q.ws.n, n);       // (more than the list holds: no longer of use)
+    __syncthreads();
+    const unsigned at = sm.bin;
+    for (unsigned i = threadIdx.x; i < n && i < 2 * NS && at + i < 2 * NS; i += NS) q.ws.list[at + i] = sm.list[i];
+}
+
+template <class T>
+__global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
+    __shared__ Shared<NS> sm;
+    const Part<T> q(p);
+    const Ask ask(p.a, q.r);
+    const u64 top = q.first(p);
+    if (!top || !(ask.T > 0.f)) {
+        if (q.part == 0) settled(p.a, q.r, top, ask);
+        return;
+    }
+    const auto d = q.draw(p, top, ask, sm);
+    u64 cut = 1ull << 32;
+    if (!plain(top, ask)) {
+        const auto l = plan_of(q, d, ask);
+        const unsigned n = q.ws.n;
+        if (l.cut && (hard(l, ask) || n > 2 * NS)) {
+            if (q.part == 0) d.from_whole(ask.k, ask.p);
+            return;
+        }
+        if (l.cut) {
+            if (l.take && q.part) return;
+            for (unsigned i = threadIdx.x; i < n; i += NS) sm.list[i] = q.ws.list[i];
+            __syncthreads();
+            if (l.take) {
+                d.from_list((int)n, l.k, ask.p, l.mass);
+                return;
+            }
+            cut = d.cut_of(l, n);
+        }
+    }
+    // every part's mass; the last workgroup to have its own draws
+    const u64 mass = block_all(d.kept_mass(q.i0, q.i1, cut, threadIdx.x, NS) * ((threadIdx.x & 63) == 0), sm, Add{});
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(&q.ws.kept[q.part], mass, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sm.n = __hip_atomic_fetch_add(&q.ws.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (sm.n != (unsigned)p.parts - 1) return;
+    const int lane = threadIdx.x & 63;
+    const u64 upto = wave_upto(lane < p.parts ? __hip_atomic_load(&q.ws.kept[lane], __ATOMIC_RELAXED,
+                                                                  __HIP_MEMORY_SCOPE_AGENT) : 0);
+    const u64 total = __shfl(upto, 63), target = d.target_of(total), past = __ballot(upto > target);
+    const int s = __ffsll(past) - 1;
+    const u64 before = s ? __shfl(upto, s - 1) : 0;
+    const int i0 = s * p.per, i1 = i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols;
+    d.from_row(i0, i1, cut, true, before, total);
+}
+
+template <class T>
+bool launch_split(const Split& p, bool cuts, hipStream_t s) {
+    const dim3 grid((unsigned)p.parts, (unsigned)p.a.rows), block(NS);
+    ACFUN_LAUNCH("k_sample_first", (k_sample_first<T>), grid, block, 0, s, p);
+    if (cuts) {
+        ACFUN_LAUNCH("k_sample_bins", (k_sample_bins<T>), grid, block, 0, s, p);
+        ACFUN_LAUNCH("k_sample_take", (k_sample_take<T>), grid, block, 0, s, p);
+    }
+    ACFUN_LAUNCH("k_sample_draw", (k_sample_draw<T>), grid, block, 0, s, p);
+    return check_launch("k_sample_draw");
+}
+
 }  // namespace
 
 bool sample_rows(const SampleArgs& a, int type, hipStream_t s) {
     int bits = 0;
     while ((1 << bits) < a.cols) ++bits;
     const int frac = 62 - bits < 48 ? 62 - bits : 48;
+    const SamplePlan plan = sample_plan(a.rows, a.cols, num_cus());
+    bool split = plan.parts > 1;
+    if (split) {
+        // a graph would keep the address of a temporary that goes back to the pool here
+        hipStreamCaptureStatus captured = hipStreamCaptureStatusNone;
+        if (!check(hipStreamIsCapturing(s, &captured), "hipStreamIsCapturing")) return false;
+        split = captured == hipStreamCaptureStatusNone;
+    }
     return with_type(type, [&](auto t) {
         using T = decltype(t);
+        if (split) {
+            Scratch ws((size_t)a.rows * sizeof(SplitRow), s);
+            return ws.p && launch_split<T>({a, frac, plan.parts, plan.per, ws.as<char>()}, a.top_k || a.top_p, s);
+        }
         if (a.cols <= kSampleShort)
             ACFUN_LAUNCH("k_sample", (k_sample<T, 256>), dim3(a.rows), dim3(256), 0, s, a, frac);
         else

@@ -165,8 +165,6 @@ struct SampleArgs {
     int* token;
     float* prob;
 };
-constexpr int kSampleMaxCols = 1 << 24, kSampleShort = 4096;
-constexpr bool sample_fits(int rows) { return launch_fits(rows, 1024); }
 bool sample_rows(const SampleArgs& a, int type, hipStream_t s);
 
 }  // namespace acfun

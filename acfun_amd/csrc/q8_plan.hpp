@@ -117,4 +117,20 @@ constexpr bool q8_rows_fit(int M, int N, int K, bool gated) {
 // in one and in two: 1 row 6.6 and 8.1, 2 rows 7.4 and 8.1, 4 rows 8.7 and 8.1, 16 rows 19 and 8.2.
 constexpr bool q8_rows_one(int M, int K) { return M <= 16 && M * (((long long)K + 511) / 512) <= 16; }
 
+// ---------------------------------------------------------------- sampling
+// A workgroup to a row, of 256 threads up to kSampleShort columns.
+constexpr int kSampleMaxCols = 1 << 24, kSampleShort = 4096;
+constexpr bool sample_fits(int rows) { return launch_fits(rows, 1024); }
+// Or `parts` workgroups with `per` columns each (whole 1024s, which are a wave's loads).
+constexpr int kSampleParts = 32;
+struct SamplePlan { int parts, per; };
+inline SamplePlan sample_plan(int rows, int cols, int cus) {
+    if (cols <= 8192 || rows > 1000000) return {1, cols};
+    int parts = (cols + 4095) / 4096;
+    if (parts > kSampleParts) parts = kSampleParts;
+    while (parts > 2 && (long long)parts * rows > 2 * cus) --parts;
+    const int per = ((cols + parts - 1) / parts + 1023) / 1024 * 1024;
+    return {(cols + per - 1) / per, per};
+}
+
 }  // namespace acfun
