@@ -97,7 +97,7 @@ template <int NT>
 struct Shared {
     static constexpr int kWaves = NT / 64, kBins = 2 * NT, kList = 2 * NT;
     u64 mass[kBins];
-    u64 list[kList];
+    u64 list[kList], some[64], some_mass[64];
     u64 part[kWaves];
     unsigned count[kBins];
     unsigned n, bin;
@@ -225,6 +225,15 @@ __device__ __forceinline__ void sort_list(u64* list, int n) {
     __syncthreads();
 }
 
+// What the histogram says of a row's first k (0: all) and p (1 or more: all): the bin that
+// the next cut lies in, and whether the tokens up to it are few enough to take them all.
+struct Plan {
+    bool by_count, cut, take;                   // cut: there is one
+    int k;
+    unsigned bin;
+    u64 need, above, mass;                      // mass: of all tokens (not by_count)
+};
+
 template <class T, int NT>
 struct Draw {
     static constexpr int kWaves = NT / 64, kBins = 2 * NT, kList = 2 * NT;
@@ -289,6 +298,30 @@ struct Draw {
         __syncthreads();
         return c;
     }
+    // The same of a bin whose tokens are among the list's n: up to 64 of them are taken out and each
+    // counts those before it; 0 if there are more.
+    __device__ __forceinline__ u64 cut_of_few(int n, unsigned b, bool mass, u64 need, u64 before) const {
+        const int t = threadIdx.x;
+        if (t == 0) sm.n = 0;
+        __syncthreads();
+        each_listed(n, [&](float x, int i) {
+            if (w.bin(x) != b) return;
+            const unsigned at = atomicAdd(&sm.n, 1u);
+            if (at < 64) sm.some[at] = place_of(x, i), sm.some_mass[at] = mass ? w(x) : 1;
+        });
+        __syncthreads();
+        const int m = (int)sm.n;
+        if (m <= 64 && t < m) {
+            const u64 mine = sm.some[t];
+#pragma unroll 4
+            for (int j = 0; j < m; ++j) before += sm.some[j] > mine ? sm.some_mass[j] : 0;
+            if (before < need && need <= before + sm.some_mass[t]) sm.above = mine;
+        }
+        __syncthreads();
+        const u64 c = m <= 64 ? sm.above : 0;
+        __syncthreads();
+        return c;
+    }
     // The part p of a mass, in steps, at least one.
     __device__ __forceinline__ u64 share(float p, u64 of) const {
         const double want = __builtin_ceil((double)p * (double)of);
@@ -302,50 +335,51 @@ struct Draw {
         *token = i;
         if (prob) *prob = (float)(w.real(x) * w.one / (double)total);
     }
-
-    // Draws from the list's n tokens, all those of the first bins: of the first k (0: all), of
-    // these the first that reach p of their mass, or of `all` (0: theirs).
-    __device__ __forceinline__ void from_list(int n, int k, float p, u64 all) const {
-        const int t = threadIdx.x;
-        sort_list<NT>(sm.list, n);
-        if (k && n > k) n = k;
-        u64 q[2], m[2], total;
+    template <class F>
+    __device__ __forceinline__ void each_listed(int n, F f) const {
 #pragma unroll 1
-        for (int pass = 0;; ++pass) {           // first in order, then by index
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                q[e] = 2 * t + e < n ? sm.list[2 * t + e] : 0;
-                m[e] = q[e] ? (pass ? w.kept(value_of((unsigned)q[e])) : w(value_of(q[e] >> 32))) : 0;
-            }
-            const u64 upto = block_upto(m[0] + m[1], sm, total), first = upto - m[1], before = first - m[0];
-            if (pass) {
-                const u64 target = target_of(total);
-                if (target == 0) break;
-                if (before <= target && target < upto) {
-                    const u64 at = target >= first ? q[1] : q[0];
-                    put(~(int)(at >> 32), value_of((unsigned)at), total);
-                }
-                return;
-            }
-            if (p < 1.f) {                      // a token is kept while those before it stay below the share
-                const u64 need = share(p, all ? all : total);
-                n = block_all((2 * t < n && before < need) + (2 * t + 1 < n && first < need), sm, Add{});
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (2 * t + e < n) sm.list[2 * t + e] = q[e] << 32 | q[e] >> 32;
-            __syncthreads();
-            sort_list<NT>(sm.list, n);
+        for (int i = threadIdx.x; i < n; i += NT) {
+            const u64 p = sm.list[i];
+            f(value_of(p >> 32), ~(int)p);
         }
-        int first = kList;                      // u = 0: the first kept, however small its weight
-#pragma unroll
-        for (int e = 1; e >= 0; --e)
-            if (2 * t + e < n) {
-                const double v = w.real(value_of((unsigned)q[e]));
-                if (v > 0. && v >= w.least) first = 2 * t + e;
-            }
-        first = block_all(first, sm, Min{});
-        if (t == 0) put(~(int)(sm.list[first] >> 32), value_of((unsigned)sm.list[first]), total);
+    }
+
+    // Draws from the list's n tokens that are not below the cut: a histogram over the index, then
+    // the tokens of a bin.
+    __device__ __forceinline__ void from_listed(int n, u64 cut) const {
+        const int t = threadIdx.x;
+        int shift = 0;
+        while ((row.cols - 1) >> shift >= kBins) ++shift;
+        clear();
+        each_listed(n, [&](float x, int i) {
+            if (place_of(x, i) >= cut) atomicAdd(&sm.mass[i >> shift], w.kept(x));
+        });
+        __syncthreads();
+        const u64 total = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{}), target = target_of(total);
+        if (target == 0) {                      // u = 0: the first kept, however small its weight
+            u64 first = ~0ull;
+            each_listed(n, [&](float x, int i) {
+                if (place_of(x, i) < cut) return;
+                const double v = w.real(x);
+                const u64 at = (u64)(unsigned)i << 32 | __float_as_uint(x);
+                if (v > 0. && v >= w.least && at < first) first = at;
+            });
+            first = block_all(first, sm, Min{});
+            if (t == 0) put((int)(first >> 32), __uint_as_float((unsigned)first), total);
+            return;
+        }
+        find_bin(sm.mass, target + 1, sm);
+        u64 before = sm.above;
+        const int i0 = (int)sm.bin << shift, i1 = i0 + (1 << shift) < row.cols ? i0 + (1 << shift) : row.cols;
+#pragma unroll 1
+        for (int i = i0; i < i1; i += NT) {
+            const float x = i + t < i1 ? (float)row.x[i + t] : -__builtin_inff();
+            const u64 v = place_of(x, i + t) >= cut ? w.kept(x) : 0;
+            u64 all;
+            const u64 upto = before + block_upto(v, sm, all);
+            if (upto > target && upto - v <= target) put(i + t, x, total);
+            before += all;
+        }
     }
 
     // The mass of the tokens a to b not below the cut, in every lane of a wave.
@@ -412,14 +446,6 @@ struct Draw {
         put(at, x, total);
     }
 
-    // What the histogram says of the row's first k (0: all) and p (1 or more: all): the bin
-    // that the next cut lies in, and whether the tokens up to it are few enough to take them all.
-    struct Plan {
-        bool by_count, cut, take;               // cut: there is one
-        int k;
-        unsigned bin;
-        u64 need, above, mass;                  // mass: of all tokens (not by_count)
-    };
     __device__ __forceinline__ Plan plan(int k, float p, bool by_count) const {
         const int t = threadIdx.x;
         Plan l{by_count, true, false, k, 0, (u64)k, 0, 0};
@@ -477,6 +503,37 @@ struct Draw {
         return cut_in_list((int)n, !l.by_count, l.need, l.above);
     }
 
+    // Draws from the list's n tokens, which are all those of the bins up to l's.
+    __device__ __forceinline__ void from_list(int n, Plan l, float p) const {
+        const bool again = l.by_count && p < 1.f;
+        unsigned bin = l.bin;
+        u64 need = l.need, above = l.above, cut;
+#pragma unroll 1
+        for (bool count = l.by_count;; count = false) {
+            cut = cut_of_few(n, bin, !count, need, above);
+            if (!cut || !count || !again) break;
+            clear();                            // p of the tokens up to the cut
+            each_listed(n, [&](float x, int i) {
+                if (place_of(x, i) >= cut) atomicAdd(&sm.mass[w.bin(x)], w(x));
+            });
+            __syncthreads();
+            need = share(p, block_all(sm.mass[2 * threadIdx.x] + sm.mass[2 * threadIdx.x + 1], sm, Add{}));
+            find_bin(sm.mass, need, sm);
+            bin = sm.bin;
+            above = sm.above;
+        }
+        if (cut == 0) {                         // many in the cut's bin: all of the list in order
+            sort_list<NT>(sm.list, n);
+            cut = cut_in_list(n, !l.by_count, l.by_count ? (u64)l.k : l.need, 0);
+            if (again) {
+                u64 mass = 0;
+                each_listed(n, [&](float x, int i) { mass += place_of(x, i) >= cut ? w(x) : 0; });
+                cut = cut_in_list(n, true, share(p, block_all(mass, sm, Add{})), 0);
+            }
+        }
+        from_listed(n, cut);
+    }
+
     // A whole row, whose largest value is w.top.
     __device__ __forceinline__ void from_whole(int k, float p) const {
         u64 cut = 1ull << 32;                   // all that can be drawn
@@ -490,7 +547,7 @@ struct Draw {
             l.take &= first;
             const unsigned n = gather(0, row.cols, l);
             if (l.take) {
-                from_list((int)n, l.k, p, l.mass);
+                from_list((int)n, l, p);
                 return;
             }
             cut = cut_of(l, n);
@@ -564,6 +621,7 @@ struct SplitRow {
     u64 first[kSampleParts], kept[kSampleParts];
     unsigned count[Shared<NS>::kBins];
     unsigned n, done;
+    Plan plan;
 };
 template <class T>
 struct Part {
@@ -616,14 +674,13 @@ __global__ __launch_bounds__(NS) void k_sample_bins(Split p) {
 
 // The row's histogram from memory, and its plan.
 template <class T>
-__device__ __forceinline__ typename Draw<T, NS>::Plan plan_of(const Part<T>& q, const Draw<T, NS>& d, const Ask& ask) {
+__device__ __forceinline__ Plan plan_of(const Part<T>& q, const Draw<T, NS>& d, const Ask& ask) {
     for (int i = threadIdx.x; i < 2 * NS; i += NS) d.sm.count[i] = q.ws.count[i], d.sm.mass[i] = q.ws.mass[i];
     __syncthreads();
     return d.plan(ask.k, ask.p, ask.k > 0);
 }
 // A top-k of many tokens with a nucleus among them: one workgroup does such a row.
-template <class L>
-__device__ __forceinline__ bool hard(const L& l, const Ask& ask) { return l.by_count && !l.take && ask.p < 1.f; }
+__device__ __forceinline__ bool hard(const Plan& l, const Ask& ask) { return l.by_count && !l.take && ask.p < 1.f; }
 
 template <class T>
 __global__ __launch_bounds__(NS) void k_sample_take(Split p) {
@@ -633,7 +690,8 @@ __global__ __launch_bounds__(NS) void k_sample_take(Split p) {
     const u64 top = q.first(p);
     if (plain(top, ask)) return;
     const auto d = q.draw(p, top, ask, sm);
-    const auto l = plan_of(q, d, ask);
+    const Plan l = plan_of(q, d, ask);
+    if (q.part == 0 && threadIdx.x == 0) q.ws.plan = l;
     if (!l.cut || hard(l, ask)) return;
     const unsigned n = d.gather(q.i0, q.i1, l);
     if (n == 0) return;
@@ -656,7 +714,7 @@ __global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
     const auto d = q.draw(p, top, ask, sm);
     u64 cut = 1ull << 32;
     if (!plain(top, ask)) {
-        const auto l = plan_of(q, d, ask);
+        const Plan l = q.ws.plan;
         const unsigned n = q.ws.n;
         if (l.cut && (hard(l, ask) || n > 2 * NS)) {
             if (q.part == 0) d.from_whole(ask.k, ask.p);
@@ -667,7 +725,7 @@ __global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
             for (unsigned i = threadIdx.x; i < n; i += NS) sm.list[i] = q.ws.list[i];
             __syncthreads();
             if (l.take) {
-                d.from_list((int)n, l.k, ask.p, l.mass);
+                d.from_list((int)n, l, ask.p);
                 return;
             }
             cut = d.cut_of(l, n);
