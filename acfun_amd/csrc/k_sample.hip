@@ -33,62 +33,87 @@ __device__ __forceinline__ float value_of(unsigned key) {
 // A token's place in the order, the first the largest.
 __device__ __forceinline__ u64 place_of(float x, int i) { return (u64)key_of(x) << 32 | (unsigned)~i; }
 
-// 2^t for t <= 0: 2^f, |f| <= 1/2, by the polynomial through 2^f at nine Chebyshev points, off by
-// 1.1e-12 of the value at most.
-__device__ __forceinline__ double exp2_of(double t) {
-    const double n = __builtin_rint(t), f = t - n;
-    double p = 0x1.63d1363a681b4p-20;
-    p = __builtin_fma(p, f, 0x1.00dc4a5344ef5p-16);
-    p = __builtin_fma(p, f, 0x1.4308ac85a69f8p-13);
-    p = __builtin_fma(p, f, 0x1.5d8745a728209p-10);
-    p = __builtin_fma(p, f, 0x1.3b2ab7181b77dp-7);
-    p = __builtin_fma(p, f, 0x1.c6b08dd6fd236p-5);
-    p = __builtin_fma(p, f, 0x1.ebfbdff823cedp-3);
-    p = __builtin_fma(p, f, 0x1.62e42fef84cf0p-1);
-    p = __builtin_fma(p, f, 1.);
-    return __builtin_amdgcn_ldexp(p, (int)n);
-}
+// A cut below all that can be drawn: the place of -infinity.
+constexpr u64 kNoCut = (u64)0x007fffff << 32 | 0xffffffffu;
+// Whether a token is not below a cut.
+struct Cut {
+    float x;
+    unsigned i;
+    __device__ __forceinline__ explicit Cut(u64 place) : x(value_of(place >> 32)), i(~(unsigned)place) {}
+    __device__ __forceinline__ bool keeps(float v, int at) const { return v > x || (v == x && (unsigned)at <= i); }
+};
+
+// 2^f, |f| <= 1/2, by the polynomial through it at nine Chebyshev points, off by 1.1e-12 of the
+// value at most.
+struct Exp2 {
+    double k[8];
+    __device__ __forceinline__ Exp2()
+        : k{0x1.62e42fef84cf0p-1, 0x1.ebfbdff823cedp-3, 0x1.c6b08dd6fd236p-5,  0x1.3b2ab7181b77dp-7,
+            0x1.5d8745a728209p-10, 0x1.4308ac85a69f8p-13, 0x1.00dc4a5344ef5p-16, 0x1.63d1363a681b4p-20} {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm("" : "+s"(k[i]));       // (or each use would copy them)
+    }
+    __device__ __forceinline__ double operator()(double f) const {
+        double p = k[7];
+#pragma unroll
+        for (int i = 6; i >= 0; --i) p = __builtin_fma(p, f, k[i]);
+        return __builtin_fma(p, f, 1.);
+    }
+};
 
 struct Weights {
-    double max, c, one, least;                  // c: log2(e) / T; one: 2^f; least: min_p
-    float top, per_2x;                          // the largest value; bins to two units of x
-    int bins;
-    // `bins` for the 50 powers of two that weigh; no infinity, whose product with 0 is none
-    __device__ __forceinline__ Weights(float largest, float T, float m, int frac, int n) {
-        max = top = largest;
-        c = 0x1.71547652b82fep+0 / (double)T;
-        one = (double)(1ull << frac);
-        least = m > 0.f ? m < 1.f ? m : 1. : 0.;
+    double max, least, c;                       // c: log2(e) / T
+    float top, half_top, per_2x;                // the largest value; bins to two units of x
+    unsigned bins;
+    int frac;
+    Exp2 exp2;
+    // `bins` for the 50 powers of two that weigh; no infinity, whose product with 0 is none.  An
+    // infinite top is the largest fp32 here, and so is what equals it; other values are far
+    // from it at any temperature.
+    __device__ __forceinline__ Weights(float largest, float T, int f, int n) {
+        const bool inf = largest == __builtin_inff();
+        top = largest;
+        half_top = 0.5f * top;
+        max = inf ? 0x1.fffffep+127 : (double)top;
+        c = inf ? 1. : 0x1.71547652b82fep+0 / (double)T;
+        least = -1000. / c;                     // (-infinity where T is infinite)
         per_2x = __builtin_fminf((float)n * (float)(0x1.715476p+0 / 25.) / T, 1e30f);
-        bins = n;
+        bins = (unsigned)n;
+        frac = f;
     }
-    // log2 of the weight; past any float's range where there is none
-    __device__ __forceinline__ double log(float x) const {
-        const double t = x == top ? 0. : ((double)x - max) * c;
-        return t > -1074. ? t : -4096.;
-    }
-    __device__ __forceinline__ double real(float x) const {
-        const double t = log(x);
-        return t > -4096. ? exp2_of(t) : 0.;
-    }
-    __device__ __forceinline__ u64 fixed(double w) const {
-        return __builtin_bit_cast(u64, __builtin_fma(w, one, 0x1p52)) - 0x4330000000000000ull;
-    }
-    // 0 past 2^-50, which rounds to no step
+    // In steps of 2^-f.  2^t = 2^n 2^f with n in the low bits of a number that has no others
+    // below 1, added to the exponent; the result's steps again in such low bits.  2^-1000 and less
+    // (-infinity, NaN) is 0 of them.
     __device__ __forceinline__ u64 operator()(float x) const {
-        const double t = log(x);
-        return t > -50. ? fixed(exp2_of(t)) : 0;
+        const double d = __builtin_fmax((double)__builtin_fminf(x, 0x1.fffffep+127f) - max, least);
+        const double z = __builtin_fma(d, c, 0x1.8p52), f = __builtin_fma(d, c, 0x1.8p52 - z);
+        const u64 p = __builtin_bit_cast(u64, exp2(f));
+        const unsigned hi = (unsigned)(p >> 32) + (((unsigned)__builtin_bit_cast(u64, z) + (unsigned)frac) << 20);
+        const double w = __builtin_bit_cast(double, (u64)hi << 32 | (unsigned)p) + 0x1p52;
+        return __builtin_bit_cast(u64, w) & 0xfffffffffffffull;
     }
-    // the same without those below min_p
-    __device__ __forceinline__ u64 kept(float x) const {
-        const double t = log(x);
-        const double w = t > -50. ? exp2_of(t) : 0.;
-        return w >= least ? fixed(w) : 0;
+    // The weight itself, however small.
+    __device__ __forceinline__ double real(float x) const {
+        const double t = __builtin_fmax(((double)__builtin_fminf(x, 0x1.fffffep+127f) - max) * c, -4096.);
+        return __builtin_amdgcn_ldexp(exp2(t - __builtin_rint(t)), (int)__builtin_rint(t));
     }
+    __device__ __forceinline__ double one() const { return __builtin_amdgcn_ldexp(1., frac); }
     // from 0 for the largest value up; `bins`: no weight (so for a NaN or -infinity)
     __device__ __forceinline__ unsigned bin(float x) const {
-        const float b = x == top ? 0.f : __builtin_fmaf(x, -0.5f, 0.5f * top) * per_2x;  // (top - x may pass fp32)
-        return b < (float)bins ? (unsigned)b : (unsigned)bins;
+        const float b = __builtin_fmaf(x, -0.5f, half_top) * per_2x;    // (top - x may pass fp32)
+        return x <= top && !(b >= (float)bins) ? (unsigned)b : bins;    // (both infinite: bin 0)
+    }
+    // The least key whose weight is m or more, in (0, 1]: 64 candidates at once.
+    __device__ __forceinline__ unsigned least_key(double m) const {
+        unsigned lo = key_of(-0x1.fffffep+127f), hi = key_of(top);
+        while (lo < hi) {
+            const unsigned lane = threadIdx.x & 63, k = lo + (unsigned)((u64)(hi - lo) * lane >> 6);
+            const u64 past = __ballot(real(value_of(k)) >= m);
+            const int s = past ? __ffsll(past) - 1 : 64;
+            if (s < 64) hi = __shfl(k, s);
+            if (s > 0) lo = __shfl(k, s - 1) + 1;
+        }
+        return hi;
     }
 };
 
@@ -104,7 +129,6 @@ struct Shared {
     u64 above;
 };
 
-struct Max { template <class V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct Min { template <class V> __device__ V operator()(V a, V b) const { return a < b ? a : b; } };
 struct Add { template <class V> __device__ V operator()(V a, V b) const { return a + b; } };
 
@@ -169,10 +193,12 @@ struct Row {
         for (int e = 0; e < V; ++e) s.v[e] = s.i + e < i ? (T)-__builtin_inff() : s.v[e];
         return s;
     }
-    // from i0 to i1, apart by whole 64 V or at the row's end, by lanes t of `threads`.  (One copy
-    // of f: what runs a few times is fetched as it runs.)
+    // from i0 to i1, apart by whole 64 V or at the row's end, by lanes t of `threads`: to
+    // f(x, i) B neighbours at once, the first one's index i.  (One copy of f for each: what runs
+    // a few times is fetched as it runs.)
+    static constexpr int B = 4;
     template <class F>
-    __device__ __forceinline__ void each(int i0, int i1, int t, int threads, F f) const {
+    __device__ __forceinline__ void fours(int i0, int i1, int t, int threads, F f) const {
         int i = i0 + t * V;
         const int step = threads * V;
         if (i >= i1) return;
@@ -183,9 +209,22 @@ struct Row {
             const bool more = i + step < i1;
             if (more) s = load(i + step);
 #pragma unroll
-            for (int e = 0; e < V; ++e) f((float)c.v[e], c.i + e);
+            for (int g = 0; g < V; g += B) {
+                float x[B];
+#pragma unroll
+                for (int e = 0; e < B; ++e) x[e] = (float)c.v[g + e];
+                f(x, c.i + g);
+            }
             if (!more) return;
         }
+    }
+    // one by one
+    template <class F>
+    __device__ __forceinline__ void each(int i0, int i1, int t, int threads, F f) const {
+        fours(i0, i1, t, threads, [&](const float (&x)[B], int i) {
+#pragma unroll
+            for (int e = 0; e < B; ++e) f(x[e], i + e);
+        });
     }
 };
 
@@ -242,8 +281,14 @@ struct Draw {
     Shared<NT>& sm;
     int* const token;
     float* const prob;
-    const float u;
+    const float u, m;                           // m: min_p
 
+    // The cut, or min_p's where that is above it.
+    __device__ __forceinline__ u64 with_floor(u64 cut) const {
+        if (!(m > 0.f)) return cut;
+        const u64 floor = (u64)w.least_key(m < 1.f ? (double)m : 1.) << 32;
+        return floor > cut ? floor : cut;
+    }
     template <class F>
     __device__ __forceinline__ void all(F f) const { row.each(0, row.cols, threadIdx.x, NT, f); }
     __device__ __forceinline__ void clear() const {
@@ -258,7 +303,7 @@ struct Draw {
     template <bool MASS>
     __device__ __forceinline__ u64 cut_by_digits(unsigned b, u64 need, u64 before) const {
         u64 prefix = 0;
-        constexpr int D = NT == 1024 ? 11 : 9;
+        constexpr int D = NT == 1024 ? 11 : NT == 512 ? 10 : 9;
         static_assert(1 << D <= kBins, "a bin to each digit");
 #pragma unroll 1
         for (int shift = 64 - D;;) {
@@ -333,7 +378,7 @@ struct Draw {
     }
     __device__ __forceinline__ void put(int i, float x, u64 total) const {
         *token = i;
-        if (prob) *prob = (float)(w.real(x) * w.one / (double)total);
+        if (prob) *prob = (float)(w.real(x) * w.one() / (double)total);
     }
     template <class F>
     __device__ __forceinline__ void each_listed(int n, F f) const {
@@ -352,17 +397,15 @@ struct Draw {
         while ((row.cols - 1) >> shift >= kBins) ++shift;
         clear();
         each_listed(n, [&](float x, int i) {
-            if (place_of(x, i) >= cut) atomicAdd(&sm.mass[i >> shift], w.kept(x));
+            if (place_of(x, i) >= cut) atomicAdd(&sm.mass[i >> shift], w(x));
         });
         __syncthreads();
         const u64 total = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{}), target = target_of(total);
         if (target == 0) {                      // u = 0: the first kept, however small its weight
             u64 first = ~0ull;
             each_listed(n, [&](float x, int i) {
-                if (place_of(x, i) < cut) return;
-                const double v = w.real(x);
                 const u64 at = (u64)(unsigned)i << 32 | __float_as_uint(x);
-                if (v > 0. && v >= w.least && at < first) first = at;
+                if (at < first && place_of(x, i) >= cut && w.real(x) > 0.) first = at;
             });
             first = block_all(first, sm, Min{});
             if (t == 0) put((int)(first >> 32), __uint_as_float((unsigned)first), total);
@@ -374,7 +417,7 @@ struct Draw {
 #pragma unroll 1
         for (int i = i0; i < i1; i += NT) {
             const float x = i + t < i1 ? (float)row.x[i + t] : -__builtin_inff();
-            const u64 v = place_of(x, i + t) >= cut ? w.kept(x) : 0;
+            const u64 v = Cut(cut).keeps(x, i + t) ? w(x) : 0;
             u64 all;
             const u64 upto = before + block_upto(v, sm, all);
             if (upto > target && upto - v <= target) put(i + t, x, total);
@@ -384,42 +427,53 @@ struct Draw {
 
     // The mass of the tokens a to b not below the cut, in every lane of a wave.
     __device__ __forceinline__ u64 kept_mass(int a, int b, u64 cut, int t, int threads) const {
+        const Cut c(cut);
         u64 mass = 0;
-        row.each(a, b, t, threads, [&](float x, int i) {
-            if (i < b && place_of(x, i) >= cut) mass += w.kept(x);
+        row.fours(a, b, t, threads, [&](const float (&x)[4], int i) {
+            u64 m[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e] = w(x[e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mass += c.keeps(x[e], i + e) ? m[e] : 0;
         });
         return wave_all(mass, Add{});
     }
+    // A wave's run of the tokens i0 to i1: whole loads of a wave.
+    static constexpr int kWaveLoad = 64 * Row<T>::V;
+    static __device__ __forceinline__ int run_of(int i0, int i1) {
+        return ((i1 - i0 + kWaves - 1) / kWaves + kWaveLoad - 1) / kWaveLoad * kWaveLoad;
+    }
     // Draws from the tokens i0 to i1 not below the cut, those before them having the mass
-    // `before` of all tokens' `total` (known: false if i0 to i1 are all tokens).
-    __device__ __forceinline__ void from_row(int i0, int i1, u64 cut, bool known, u64 before, u64 total) const {
-        constexpr int Q = 64 * Row<T>::V;       // a wave's values at once
+    // `before` of all tokens' `total` (0: it is that of these).  `runs`: sm.part has the masses of
+    // the waves' runs.
+    __device__ __forceinline__ void from_row(int i0, int i1, u64 cut, u64 before, u64 total, bool runs) const {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        u64 target = known ? target_of(total) : 1;
+        u64 target = total ? target_of(total) : 1;
         // a run to each wave, then a part of the run that the target falls in
 #pragma unroll 1
-        while (target) {
-            const int per = ((i1 - i0 + kWaves - 1) / kWaves + Q - 1) / Q * Q;
-            const int a = i0 + wave * per < i1 ? i0 + wave * per : i1, b = a + per < i1 ? a + per : i1;
-            const u64 mass = kept_mass(a, b, cut, lane, 64);
-            if (lane == 0) sm.part[wave] = mass;
-            __syncthreads();
+        for (; target; runs = false) {
+            const int per = run_of(i0, i1);
+            if (!runs) {
+                const int a = i0 + wave * per < i1 ? i0 + wave * per : i1, b = a + per < i1 ? a + per : i1;
+                const u64 mass = kept_mass(a, b, cut, lane, 64);
+                if (lane == 0) sm.part[wave] = mass;
+                __syncthreads();
+            }
             const u64 upto = wave_upto(lane < kWaves ? sm.part[lane % kWaves] : 0);
-            if (!known) total = __shfl(upto, kWaves - 1), target = target_of(total), known = true;
+            if (!total) total = __shfl(upto, kWaves - 1), target = target_of(total);
             const u64 past = __ballot(lane < kWaves && before + upto > target);
             const int s = past ? __ffsll(past) - 1 : kWaves - 1;
             before += s ? __shfl(upto, s - 1) : 0;
             __syncthreads();
             i0 += s * per;
             i1 = i0 + per < i1 ? i0 + per : i1;
-            if (per == Q) break;
+            if (per == kWaveLoad) break;
         }
         if (target == 0) {                      // u = 0: the first kept, however small its weight
+            const Cut c(cut);
             int first = row.cols;
             all([&](float x, int i) {
-                if (i >= first || place_of(x, i) < cut) return;
-                const double v = w.real(x);
-                if (v > 0. && v >= w.least) first = i;
+                if (i < first && c.keeps(x, i) && w.real(x) > 0.) first = i;
             });
             __syncthreads();
             first = block_all(first, sm, Min{});
@@ -431,7 +485,7 @@ struct Draw {
         u64 m[Row<T>::V], mine = 0;
 #pragma unroll
         for (int e = 0; e < Row<T>::V; ++e) {
-            m[e] = v.i + e < i1 && place_of((float)v.v[e], v.i + e) >= cut ? w.kept((float)v.v[e]) : 0;
+            m[e] = v.i + e < i1 && Cut(cut).keeps((float)v.v[e], v.i + e) ? w((float)v.v[e]) : 0;
             mine += m[e];
         }
         before += wave_upto(mine) - mine;
@@ -471,29 +525,63 @@ struct Draw {
     }
     // The histogram of the tokens i0 to i1 not below the cut.
     __device__ __forceinline__ void fill(int i0, int i1, bool count, bool mass, u64 cut) const {
-        row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) {
-            const unsigned b = w.bin(x);
-            if (b >= (unsigned)kBins || i >= i1 || (cut >> 32 && place_of(x, i) < cut)) return;
-            if (count) atomicAdd(&sm.count[b], 1u);
-            if (mass) atomicAdd(&sm.mass[b], w(x));
+        const Cut c(cut);
+        row.fours(i0, i1, threadIdx.x, NT, [&](const float (&x)[4], int i) {
+            u64 m[4] = {};
+            if (mass)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m[e] = w(x[e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned b = w.bin(x[e]);
+                if (b >= (unsigned)kBins || !c.keeps(x[e], i + e)) continue;
+                if (count) atomicAdd(&sm.count[b], 1u);
+                if (mass) atomicAdd(&sm.mass[b], m[e]);
+            }
         });
         __syncthreads();
     }
-    // Tokens i0 to i1 of the bins up to l's (l.take) or of that alone to the list; their number.
-    __device__ __forceinline__ unsigned gather(int i0, int i1, const Plan& l) const {
+    // One pass over the tokens i0 to i1, a run to each wave.  To the list: those of the bins up
+    // to l's (l.take), or of that alone; their number is the result.  To sm.part (MASS): the
+    // masses of the runs' tokens before that bin, or of all (not l.cut), without those below `floor`.
+    template <bool MASS>
+    __device__ __forceinline__ unsigned sweep(int i0, int i1, const Plan& l, u64 floor) const {
         if (threadIdx.x == 0) sm.n = 0;
         __syncthreads();
-        const unsigned b0 = l.take ? 0 : l.bin;
-        row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) {
-            const unsigned b = w.bin(x);
-            if (b < b0 || b > l.bin || i >= i1) return;
-            const unsigned at = atomicAdd(&sm.n, 1u);
-            if (at < (unsigned)kList) sm.list[at] = place_of(x, i);
+        const int per = run_of(i0, i1), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const int a = i0 + wave * per < i1 ? i0 + wave * per : i1, b = a + per < i1 ? a + per : i1;
+        const unsigned b0 = l.take ? 0 : l.bin, b1 = l.cut ? l.bin : (unsigned)kBins;
+        const Cut c(floor);
+        u64 mass = 0;
+        row.fours(a, b, lane, 64, [&](const float (&x)[4], int i) {
+            u64 m[4] = {};
+            if constexpr (MASS)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m[e] = w(x[e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned at = w.bin(x[e]);
+                if (MASS) mass += at < b1 && c.keeps(x[e], i + e) ? m[e] : 0;
+                if (at < b0 || at > b1 || !l.cut) continue;
+                const unsigned n = atomicAdd(&sm.n, 1u);
+                if (n < (unsigned)kList) sm.list[n] = place_of(x[e], i + e);
+            }
         });
+        if constexpr (MASS) {
+            mass = wave_all(mass, Add{});
+            if (lane == 0) sm.part[wave] = mass;
+        }
         __syncthreads();
         const unsigned n = sm.n;
         __syncthreads();
         return n;
+    }
+    // The list's tokens not below the cut, to the masses of the runs of i0 to i1.
+    __device__ __forceinline__ void add_list(int n, u64 cut, int i0, int per, u64* masses) const {
+        each_listed(n, [&](float x, int i) {
+            if (place_of(x, i) >= cut) atomicAdd(&masses[(i - i0) / per], w(x));
+        });
+        __syncthreads();
     }
     // The cut of l, from the list's n tokens of its bin (more than it holds: from the row).
     __device__ __forceinline__ u64 cut_of(const Plan& l, unsigned n) const {
@@ -531,44 +619,57 @@ struct Draw {
                 cut = cut_in_list(n, true, share(p, block_all(mass, sm, Add{})), 0);
             }
         }
-        from_listed(n, cut);
+        from_listed(n, with_floor(cut));
     }
 
     // A whole row, whose largest value is w.top.
     __device__ __forceinline__ void from_whole(int k, float p) const {
-        u64 cut = 1ull << 32;                   // all that can be drawn
-        bool by_count = k > 0;
+        const bool nucleus = p < 1.f;
+        const u64 floor = with_floor(kNoCut);
+        u64 cut = kNoCut;
+        Plan l{};
 #pragma unroll 1
-        for (bool first = true; by_count || p < 1.f; first = false) {
+        for (bool first = true; k > 0 || nucleus; first = false) {
             clear();
-            fill(0, row.cols, first, p < 1.f, first ? 0 : cut);
-            Plan l = plan(k, p, by_count);
+            fill(0, row.cols, first, nucleus, cut);
+            l = plan(first ? k : 0, p, first && k > 0);
             if (!l.cut) break;
             l.take &= first;
-            const unsigned n = gather(0, row.cols, l);
-            if (l.take) {
-                from_list((int)n, l, p);
-                return;
+            if (l.by_count && nucleus && !l.take) {             // a cut by number, then p of the tokens up to it
+                cut = cut_of(l, sweep<false>(0, row.cols, l, floor));
+                continue;
             }
-            cut = cut_of(l, n);
-            if (!l.by_count || !(p < 1.f)) break;
-            by_count = false;                   // p of the tokens up to the cut
+            break;
         }
-        from_row(0, row.cols, cut, false, 0, 0);
+        if (l.take) {
+            const int n = (int)sweep<false>(0, row.cols, l, floor);
+            from_list(n, l, p);
+            return;
+        }
+        bool runs = false;
+        if (l.cut) {
+            const unsigned n = sweep<true>(0, row.cols, l, floor);
+            runs = n <= (unsigned)kList;
+            const u64 mine = sm.part[threadIdx.x % kWaves];     // (what finds the cut uses them)
+            __syncthreads();
+            cut = cut_of(l, n);
+            cut = cut > floor ? cut : floor;
+            if (threadIdx.x < kWaves) sm.part[threadIdx.x] = mine;
+            __syncthreads();
+            if (runs) add_list((int)n, cut, 0, run_of(0, row.cols), sm.part);
+        } else {
+            cut = floor;
+        }
+        from_row(0, row.cols, cut, 0, 0, runs);
     }
 };
 
-// A row's largest value with its lowest index, as its place; 0 for a row with nothing to draw.
+// The largest value; -infinity for a row with nothing to draw.
 template <int NT, class T>
-__device__ __forceinline__ u64 first_of(const Row<T>& row, int i0, int i1, Shared<NT>& sm) {
+__device__ __forceinline__ float largest_of(const Row<T>& row, int i0, int i1, Shared<NT>& sm) {
     float top = -__builtin_inff();
-    int at = 0;
-    row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) {
-        const bool more = x > top && i < i1;
-        top = more ? x : top;
-        at = more ? i : at;
-    });
-    return block_all(top > -__builtin_inff() ? place_of(top, at) : 0, sm, Max{});
+    row.each(i0, i1, threadIdx.x, NT, [&](float x, int) { top = __builtin_fmaxf(top, x); });
+    return block_all(top, sm, [](float p, float q) { return __builtin_fmaxf(p, q); });
 }
 // What a row asks for.
 struct Ask {
@@ -583,15 +684,18 @@ struct Ask {
         if (k < 0 || k >= a.cols) k = 0;
     }
 };
-// A row that needs no draw: nothing in it, or the largest asked for.
-__device__ __forceinline__ bool settled(const SampleArgs& a, int r, u64 first, const Ask& ask) {
-    if (first && ask.T > 0.f) return false;
+// A row that needs no draw: nothing in it, or the largest asked for, of which i0 to i1 hold the first.
+template <int NT, class T>
+__device__ __forceinline__ void settle(const SampleArgs& a, int r, const Row<T>& row, float top, int i0, int i1, Shared<NT>& sm) {
+    int first = a.cols;
+    if (top > -__builtin_inff()) row.each(i0, i1, threadIdx.x, NT, [&](float x, int i) { first = x == top && i < first ? i : first; });
+    first = block_all(first, sm, Min{});
     if (threadIdx.x == 0) {
-        a.token[r] = first ? ~(int)first : -1;
-        if (a.prob) a.prob[r] = first ? 1.f : 0.f;
+        a.token[r] = first < a.cols ? first : -1;
+        if (a.prob) a.prob[r] = first < a.cols ? 1.f : 0.f;
     }
-    return true;
 }
+__device__ __forceinline__ bool settled(float top, const Ask& ask) { return !(top > -__builtin_inff()) || !(ask.T > 0.f); }
 
 // A workgroup to a row, which it reads three to five times.
 template <class T, int NT>
@@ -600,10 +704,13 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a, int frac) {
     const int r = blockIdx.x;
     const Row<T> row{(const T*)a.x + (size_t)r * a.ld, a.cols};
     const Ask ask(a, r);
-    const u64 first = first_of(row, 0, a.cols, sm);
-    if (settled(a, r, first, ask)) return;
-    const Draw<T, NT> d{row, Weights(value_of(first >> 32), ask.T, ask.m, frac, 2 * NT), sm, a.token + r,
-                        a.prob ? a.prob + r : nullptr, ask.u};
+    const float top = largest_of(row, 0, a.cols, sm);
+    if (settled(top, ask)) {
+        settle(a, r, row, top, 0, a.cols, sm);
+        return;
+    }
+    const Draw<T, NT> d{row, Weights(top, ask.T, frac, 2 * NT), sm, a.token + r, a.prob ? a.prob + r : nullptr, ask.u,
+                        ask.m};
     d.from_whole(ask.k, ask.p);
 }
 
@@ -618,9 +725,10 @@ struct Split {
 constexpr int NS = 1024;                        // threads
 struct SplitRow {
     u64 mass[Shared<NS>::kBins], list[Shared<NS>::kList];
-    u64 first[kSampleParts], kept[kSampleParts];
+    u64 kept[kSampleParts];
+    float top[kSampleParts];
     unsigned count[Shared<NS>::kBins];
-    unsigned n, done;
+    unsigned n;
     Plan plan;
 };
 template <class T>
@@ -631,18 +739,23 @@ struct Part {
     __device__ __forceinline__ explicit Part(const Split& p)
         : r(blockIdx.y), part(blockIdx.x), i0(part * p.per), i1(i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols),
           row{(const T*)p.a.x + (size_t)r * p.a.ld, p.a.cols}, ws(((SplitRow*)p.rows)[r]) {}
-    __device__ __forceinline__ u64 first(const Split& p) const {
+    __device__ __forceinline__ float top(const Split& p) const {
         const int lane = threadIdx.x & 63;
-        return wave_all(lane < p.parts ? ws.first[lane] : 0, Max{});
+        return wave_all(lane < p.parts ? ws.top[lane] : -__builtin_inff(), [](float p, float q) { return __builtin_fmaxf(p, q); });
     }
-    __device__ __forceinline__ Draw<T, NS> draw(const Split& p, u64 top, const Ask& ask, Shared<NS>& sm) const {
-        return {row, Weights(value_of(top >> 32), ask.T, ask.m, p.frac, 2 * NS), sm, p.a.token + r,
-                p.a.prob ? p.a.prob + r : nullptr, ask.u};
+    // the first part that holds the row's largest
+    __device__ __forceinline__ int of_top(const Split& p, float top) const {
+        const int lane = threadIdx.x & 63;
+        return __ffsll(__ballot(lane < p.parts && ws.top[lane] == top)) - 1;
+    }
+    __device__ __forceinline__ Draw<T, NS> draw(const Split& p, float top, const Ask& ask, Shared<NS>& sm) const {
+        return {row, Weights(top, ask.T, p.frac, 2 * NS), sm, p.a.token + r, p.a.prob ? p.a.prob + r : nullptr, ask.u,
+                ask.m};
     }
 };
 // Those that are settled without a histogram.
-__device__ __forceinline__ bool plain(u64 top, const Ask& ask) {
-    return !top || !(ask.T > 0.f) || (!ask.k && !(ask.p < 1.f));
+__device__ __forceinline__ bool plain(float top, const Ask& ask) {
+    return settled(top, ask) || (!ask.k && !(ask.p < 1.f));
 }
 
 template <class T>
@@ -650,9 +763,9 @@ __global__ __launch_bounds__(NS) void k_sample_first(Split p) {
     __shared__ Shared<NS> sm;
     const Part<T> q(p);
     for (int i = q.part * NS + threadIdx.x; i < 2 * NS; i += p.parts * NS) q.ws.mass[i] = 0, q.ws.count[i] = 0;
-    if (q.part == 0 && threadIdx.x == 0) q.ws.n = 0, q.ws.done = 0;
-    const u64 top = first_of(q.row, q.i0, q.i1, sm);
-    if (threadIdx.x == 0) q.ws.first[q.part] = top;
+    if (q.part == 0 && threadIdx.x == 0) q.ws.n = 0;
+    const float top = largest_of(q.row, q.i0, q.i1, sm);
+    if (threadIdx.x == 0) q.ws.top[q.part] = top;
 }
 
 template <class T>
@@ -660,11 +773,11 @@ __global__ __launch_bounds__(NS) void k_sample_bins(Split p) {
     __shared__ Shared<NS> sm;
     const Part<T> q(p);
     const Ask ask(p.a, q.r);
-    const u64 top = q.first(p);
+    const float top = q.top(p);
     if (plain(top, ask)) return;
     const auto d = q.draw(p, top, ask, sm);
     d.clear();
-    d.fill(q.i0, q.i1, true, ask.p < 1.f, 0);
+    d.fill(q.i0, q.i1, true, ask.p < 1.f, kNoCut);
 #pragma unroll
     for (int i = threadIdx.x; i < 2 * NS; i += NS) {
         if (sm.count[i]) atomicAdd(&q.ws.count[i], sm.count[i]);
@@ -687,77 +800,82 @@ __global__ __launch_bounds__(NS) void k_sample_take(Split p) {
     __shared__ Shared<NS> sm;
     const Part<T> q(p);
     const Ask ask(p.a, q.r);
-    const u64 top = q.first(p);
-    if (plain(top, ask)) return;
+    const float top = q.top(p);
+    if (settled(top, ask)) return;
     const auto d = q.draw(p, top, ask, sm);
-    const Plan l = plan_of(q, d, ask);
-    if (q.part == 0 && threadIdx.x == 0) q.ws.plan = l;
-    if (!l.cut || hard(l, ask)) return;
-    const unsigned n = d.gather(q.i0, q.i1, l);
-    if (n == 0) return;
-    if (threadIdx.x == 0) sm.bin = atomicAdd(&q.ws.n, n);       // (more than the list holds: no longer of use)
+    Plan l{};
+    if (!plain(top, ask)) {
+        l = plan_of(q, d, ask);
+        if (q.part == 0 && threadIdx.x == 0) q.ws.plan = l;
+        if (hard(l, ask)) return;
+    }
+    unsigned n = 0;
+    u64 mass = 0;
+    if (l.take) {
+        n = d.template sweep<false>(q.i0, q.i1, l, 0);
+    } else {
+        n = d.template sweep<true>(q.i0, q.i1, l, d.with_floor(kNoCut));
+        mass = block_all((threadIdx.x & 63) == 0 ? sm.part[threadIdx.x >> 6] : 0, sm, Add{});
+    }
+    if (threadIdx.x == 0) {
+        q.ws.kept[q.part] = mass;
+        sm.bin = n ? atomicAdd(&q.ws.n, n) : 0;                 // (more than the list holds: no longer of use)
+    }
     __syncthreads();
     const unsigned at = sm.bin;
     for (unsigned i = threadIdx.x; i < n && i < 2 * NS && at + i < 2 * NS; i += NS) q.ws.list[at + i] = sm.list[i];
 }
 
+// A workgroup to a row.
 template <class T>
 __global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
     __shared__ Shared<NS> sm;
+    __shared__ u64 kept[kSampleParts];
     const Part<T> q(p);
     const Ask ask(p.a, q.r);
-    const u64 top = q.first(p);
-    if (!top || !(ask.T > 0.f)) {
-        if (q.part == 0) settled(p.a, q.r, top, ask);
+    const float top = q.top(p);
+    if (settled(top, ask)) {
+        const int i0 = q.of_top(p, top) * p.per;                // (-1: there is none)
+        settle(p.a, q.r, q.row, top, i0, i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols, sm);
         return;
     }
     const auto d = q.draw(p, top, ask, sm);
-    u64 cut = 1ull << 32;
-    if (!plain(top, ask)) {
-        const Plan l = q.ws.plan;
-        const unsigned n = q.ws.n;
-        if (l.cut && (hard(l, ask) || n > 2 * NS)) {
-            if (q.part == 0) d.from_whole(ask.k, ask.p);
-            return;
-        }
-        if (l.cut) {
-            if (l.take && q.part) return;
-            for (unsigned i = threadIdx.x; i < n; i += NS) sm.list[i] = q.ws.list[i];
-            __syncthreads();
-            if (l.take) {
-                d.from_list((int)n, l, ask.p);
-                return;
-            }
-            cut = d.cut_of(l, n);
-        }
+    const Plan l = plain(top, ask) ? Plan{} : q.ws.plan;
+    const unsigned n = q.ws.n;
+    if (l.cut && (hard(l, ask) || n > 2 * NS)) {
+        d.from_whole(ask.k, ask.p);
+        return;
     }
-    // every part's mass; the last workgroup to have its own draws
-    const u64 mass = block_all(d.kept_mass(q.i0, q.i1, cut, threadIdx.x, NS) * ((threadIdx.x & 63) == 0), sm, Add{});
-    if (threadIdx.x == 0) {
-        __hip_atomic_store(&q.ws.kept[q.part], mass, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sm.n = __hip_atomic_fetch_add(&q.ws.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    if ((int)threadIdx.x < p.parts) kept[threadIdx.x] = q.ws.kept[threadIdx.x];
+    if (l.cut)
+        for (unsigned i = threadIdx.x; i < n; i += NS) sm.list[i] = q.ws.list[i];
     __syncthreads();
-    if (sm.n != (unsigned)p.parts - 1) return;
+    if (l.take) {
+        d.from_list((int)n, l, ask.p);
+        return;
+    }
+    u64 cut = d.with_floor(kNoCut);
+    if (l.cut) {
+        const u64 c = d.cut_of(l, n);
+        cut = c > cut ? c : cut;
+        d.add_list((int)n, cut, 0, p.per, kept);
+    }
     const int lane = threadIdx.x & 63;
-    const u64 upto = wave_upto(lane < p.parts ? __hip_atomic_load(&q.ws.kept[lane], __ATOMIC_RELAXED,
-                                                                  __HIP_MEMORY_SCOPE_AGENT) : 0);
+    const u64 upto = wave_upto(lane < p.parts ? kept[lane] : 0);
     const u64 total = __shfl(upto, 63), target = d.target_of(total), past = __ballot(upto > target);
     const int s = __ffsll(past) - 1;
     const u64 before = s ? __shfl(upto, s - 1) : 0;
-    const int i0 = s * p.per, i1 = i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols;
-    d.from_row(i0, i1, cut, true, before, total);
+    const int i0 = s * p.per;
+    d.from_row(i0, i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols, cut, before, total, false);
 }
 
 template <class T>
 bool launch_split(const Split& p, bool cuts, hipStream_t s) {
     const dim3 grid((unsigned)p.parts, (unsigned)p.a.rows), block(NS);
     ACFUN_LAUNCH("k_sample_first", (k_sample_first<T>), grid, block, 0, s, p);
-    if (cuts) {
-        ACFUN_LAUNCH("k_sample_bins", (k_sample_bins<T>), grid, block, 0, s, p);
-        ACFUN_LAUNCH("k_sample_take", (k_sample_take<T>), grid, block, 0, s, p);
-    }
-    ACFUN_LAUNCH("k_sample_draw", (k_sample_draw<T>), grid, block, 0, s, p);
+    if (cuts) ACFUN_LAUNCH("k_sample_bins", (k_sample_bins<T>), grid, block, 0, s, p);
+    ACFUN_LAUNCH("k_sample_take", (k_sample_take<T>), grid, block, 0, s, p);
+    ACFUN_LAUNCH("k_sample_draw", (k_sample_draw<T>), dim3(1, (unsigned)p.a.rows), block, 0, s, p);
     return check_launch("k_sample_draw");
 }
 
@@ -781,8 +899,10 @@ bool sample_rows(const SampleArgs& a, int type, hipStream_t s) {
             Scratch ws((size_t)a.rows * sizeof(SplitRow), s);
             return ws.p && launch_split<T>({a, frac, plan.parts, plan.per, ws.as<char>()}, a.top_k || a.top_p, s);
         }
-        if (a.cols <= kSampleShort)
+        if (plan.threads == 256)
             ACFUN_LAUNCH("k_sample", (k_sample<T, 256>), dim3(a.rows), dim3(256), 0, s, a, frac);
+        else if (plan.threads == 512)
+            ACFUN_LAUNCH("k_sample", (k_sample<T, 512>), dim3(a.rows), dim3(512), 0, s, a, frac);
         else
             ACFUN_LAUNCH("k_sample", (k_sample<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a, frac);
         return check_launch("k_sample");

@@ -118,19 +118,18 @@ constexpr bool q8_rows_fit(int M, int N, int K, bool gated) {
 constexpr bool q8_rows_one(int M, int K) { return M <= 16 && M * (((long long)K + 511) / 512) <= 16; }
 
 // ---------------------------------------------------------------- sampling
-// A workgroup to a row, of 256 threads up to kSampleShort columns.
-constexpr int kSampleMaxCols = 1 << 24, kSampleShort = 4096;
+// A workgroup of `threads` to a row, or `parts` of 1024 with `per` columns each (whole
+// 1024s, which are two waves' loads).
+constexpr int kSampleMaxCols = 1 << 24, kSampleParts = 32;
 constexpr bool sample_fits(int rows) { return launch_fits(rows, 1024); }
-// Or `parts` workgroups with `per` columns each (whole 1024s, which are a wave's loads).
-constexpr int kSampleParts = 32;
-struct SamplePlan { int parts, per; };
+struct SamplePlan { int parts, per, threads; };
 inline SamplePlan sample_plan(int rows, int cols, int cus) {
-    if (cols <= 8192 || rows > 1000000) return {1, cols};
+    if (cols <= 8192 || rows > 1000000) return {1, cols, cols <= 1024 ? 256 : cols <= 8192 ? 512 : 1024};
     int parts = (cols + 4095) / 4096;
     if (parts > kSampleParts) parts = kSampleParts;
     while (parts > 2 && (long long)parts * rows > 2 * cus) --parts;
     const int per = ((cols + parts - 1) / parts + 1023) / 1024 * 1024;
-    return {(cols + per - 1) / per, per};
+    return {(cols + per - 1) / per, per, 1024};
 }
 
 }  // namespace acfun
