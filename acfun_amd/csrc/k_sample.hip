@@ -117,18 +117,22 @@ struct Weights {
     }
 };
 
+// Up to so many tokens of a bin count those before them, each all the others.
+constexpr int kSome = 256;
+
 // A workgroup's: two bins and two entries of the list to a thread.
 template <int NT>
 struct Shared {
     static constexpr int kWaves = NT / 64, kBins = 2 * NT, kList = 2 * NT;
     u64 mass[kBins];
-    u64 list[kList], some[64], some_mass[64];
+    u64 list[kList], some[kSome], some_mass[kSome], some_before[kSome];
     u64 part[kWaves];
     unsigned count[kBins];
     unsigned n, bin;
     u64 above;
 };
 
+struct Max { template <class V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct Min { template <class V> __device__ V operator()(V a, V b) const { return a < b ? a : b; } };
 struct Add { template <class V> __device__ V operator()(V a, V b) const { return a + b; } };
 
@@ -246,24 +250,6 @@ __device__ __forceinline__ bool find_bin(const V* bins, u64 need, Shared<NT>& sm
     return sm.bin < 2 * NT;
 }
 
-// The list's first n entries, the largest first; the rest of it up to a power of two is 0.
-template <int NT>
-__device__ __forceinline__ void sort_list(u64* list, int n) {
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += NT) list[i] = 0;
-    for (int run = 2; run <= size; run *= 2)
-        for (int d = run / 2; d > 0; d /= 2) {
-            __syncthreads();
-            const int t = threadIdx.x, i = (t & ~(d - 1)) * 2 + (t & (d - 1));
-            if (t < size / 2) {
-                const u64 a = list[i], b = list[i + d];
-                if ((a < b) == ((i & run) == 0)) list[i] = b, list[i + d] = a;
-            }
-        }
-    __syncthreads();
-}
-
 // What the histogram says of a row's first k (0: all) and p (1 or more: all): the bin that
 // the next cut lies in, and whether the tokens up to it are few enough to take them all.
 struct Plan {
@@ -327,43 +313,62 @@ struct Draw {
             shift = shift > D ? shift - D : 0;
         }
     }
-    // The same of a bin whose tokens are the list's n, in order.
-    __device__ __forceinline__ u64 cut_in_list(int n, bool mass, u64 need, u64 before) const {
+    // The same of a bin whose tokens are among the list's n.  While they are more than kSome, a
+    // histogram over their places narrows them; then each adds up those before it, with
+    // NT / kSome threads.
+    __device__ __forceinline__ u64 cut_in_list(int n, unsigned b, bool mass, u64 need, u64 before) const {
         const int t = threadIdx.x;
-        u64 p[2], m[2], total;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            p[e] = 2 * t + e < n ? sm.list[2 * t + e] : 0;
-            m[e] = !p[e] ? 0 : mass ? w(value_of(p[e] >> 32)) : 1;
+        u64 lo = 0, hi = ~0ull;
+        unsigned m;
+#pragma unroll 1
+        for (;;) {
+            if (t == 0) sm.n = 0;
+            if (t < kSome) sm.some_before[t] = 0;
+            __syncthreads();
+            u64 least = ~0ull, most = 0;
+            each_listed(n, [&](float x, int i) {
+                const u64 p = place_of(x, i);
+                if (w.bin(x) != b || p < lo || p > hi) return;
+                const unsigned at = atomicAdd(&sm.n, 1u);
+                if (at < (unsigned)kSome) sm.some[at] = p, sm.some_mass[at] = mass ? w(x) : 1;
+                least = p < least ? p : least;
+                most = p > most ? p : most;
+            });
+            __syncthreads();
+            m = sm.n;
+            if (m <= (unsigned)kSome) break;
+            lo = block_all(least, sm, Min{});
+            hi = block_all(most, sm, Max{});
+            int shift = 0;
+            while ((hi - lo) >> shift >= (u64)kBins) ++shift;
+            clear();
+            each_listed(n, [&](float x, int i) {
+                const u64 p = place_of(x, i);
+                if (p >= lo && p <= hi) atomicAdd(&sm.mass[(hi - p) >> shift], mass ? w(x) : 1ull);
+            });
+            __syncthreads();
+            find_bin(sm.mass, need - before, sm);
+            before += sm.above;
+            hi -= (u64)sm.bin << shift;
+            const u64 last = (1ull << shift) - 1;
+            lo = hi - lo > last ? hi - last : lo;
+            __syncthreads();
         }
-        const u64 upto = before + block_upto(m[0] + m[1], sm, total), first = upto - m[1];
-        if (first - m[0] < need && need <= upto) sm.above = first >= need ? p[0] : p[1];
+        const int e = t % kSome;
+        const u64 mine = e < (int)m ? sm.some[e] : 0;
+        if (mine) {
+            u64 sum = 0;
+#pragma unroll 2
+            for (int j = t / kSome; j < (int)m; j += NT / kSome) sum += sm.some[j] > mine ? sm.some_mass[j] : 0;
+            if (sum) atomicAdd(&sm.some_before[e], sum);
+        }
         __syncthreads();
-        const u64 c = sm.above;
-        __syncthreads();
-        return c;
-    }
-    // The same of a bin whose tokens are among the list's n: up to 64 of them are taken out and each
-    // counts those before it; 0 if there are more.
-    __device__ __forceinline__ u64 cut_of_few(int n, unsigned b, bool mass, u64 need, u64 before) const {
-        const int t = threadIdx.x;
-        if (t == 0) sm.n = 0;
-        __syncthreads();
-        each_listed(n, [&](float x, int i) {
-            if (w.bin(x) != b) return;
-            const unsigned at = atomicAdd(&sm.n, 1u);
-            if (at < 64) sm.some[at] = place_of(x, i), sm.some_mass[at] = mass ? w(x) : 1;
-        });
-        __syncthreads();
-        const int m = (int)sm.n;
-        if (m <= 64 && t < m) {
-            const u64 mine = sm.some[t];
-#pragma unroll 4
-            for (int j = 0; j < m; ++j) before += sm.some[j] > mine ? sm.some_mass[j] : 0;
+        if (t < (int)m) {
+            before += sm.some_before[t];
             if (before < need && need <= before + sm.some_mass[t]) sm.above = mine;
         }
         __syncthreads();
-        const u64 c = m <= 64 ? sm.above : 0;
+        const u64 c = sm.above;
         __syncthreads();
         return c;
     }
@@ -412,8 +417,27 @@ struct Draw {
             return;
         }
         find_bin(sm.mass, target + 1, sm);
+        const unsigned bin = sm.bin;
         u64 before = sm.above;
-        const int i0 = (int)sm.bin << shift, i1 = i0 + (1 << shift) < row.cols ? i0 + (1 << shift) : row.cols;
+        if (t == 0) sm.n = 0;
+        __syncthreads();
+        each_listed(n, [&](float x, int i) {
+            if ((unsigned)i >> shift != bin || place_of(x, i) < cut) return;
+            const unsigned at = atomicAdd(&sm.n, 1u);
+            if (at < kSome) sm.some[at] = (u64)(unsigned)i << 32 | __float_as_uint(x), sm.some_mass[at] = w(x);
+        });
+        __syncthreads();
+        const int m = (int)sm.n;
+        if (m <= kSome) {
+            if (t >= m) return;
+            const u64 mine = sm.some[t];
+#pragma unroll 1
+            for (int j = 0; j < m; ++j) before += sm.some[j] < mine ? sm.some_mass[j] : 0;
+            if (before <= target && target < before + sm.some_mass[t])
+                put((int)(mine >> 32), __uint_as_float((unsigned)mine), total);
+            return;
+        }
+        const int i0 = (int)bin << shift, i1 = i0 + (1 << shift) < row.cols ? i0 + (1 << shift) : row.cols;
 #pragma unroll 1
         for (int i = i0; i < i1; i += NT) {
             const float x = i + t < i1 ? (float)row.x[i + t] : -__builtin_inff();
@@ -503,21 +527,19 @@ struct Draw {
     __device__ __forceinline__ Plan plan(int k, float p, bool by_count) const {
         const int t = threadIdx.x;
         Plan l{by_count, true, false, k, 0, (u64)k, 0, 0};
-        if (by_count && !find_bin(sm.count, l.need, sm)) {      // fewer tokens than k that weigh anything: no limit
-            l.k = 0, l.by_count = false;
-            __syncthreads();
-        }
-        if (!l.by_count) {
-            if (!(p < 1.f)) {
-                l.cut = false;
-                return l;
-            }
+        if (by_count) {                         // (fewer tokens than k that weigh anything: no limit)
+            l.cut = find_bin(sm.count, l.need, sm);
+        } else if (p < 1.f) {
             l.mass = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{});
             l.need = share(p, l.mass);
             find_bin(sm.mass, l.need, sm);
+        } else {
+            l.cut = false;
         }
         l.bin = sm.bin;
         l.above = sm.above;
+        __syncthreads();
+        if (!l.cut) return l;
         const unsigned few =
             (2 * t <= (int)l.bin ? sm.count[2 * t] : 0) + (2 * t + 1 <= (int)l.bin ? sm.count[2 * t + 1] : 0);
         l.take = block_all(few, sm, Add{}) <= (unsigned)kList;
@@ -587,8 +609,7 @@ struct Draw {
     __device__ __forceinline__ u64 cut_of(const Plan& l, unsigned n) const {
         if (n > (unsigned)kList)
             return l.by_count ? cut_by_digits<false>(l.bin, l.need, l.above) : cut_by_digits<true>(l.bin, l.need, l.above);
-        sort_list<NT>(sm.list, (int)n);
-        return cut_in_list((int)n, !l.by_count, l.need, l.above);
+        return cut_in_list((int)n, l.bin, !l.by_count, l.need, l.above);
     }
 
     // Draws from the list's n tokens, which are all those of the bins up to l's.
@@ -598,8 +619,8 @@ struct Draw {
         u64 need = l.need, above = l.above, cut;
 #pragma unroll 1
         for (bool count = l.by_count;; count = false) {
-            cut = cut_of_few(n, bin, !count, need, above);
-            if (!cut || !count || !again) break;
+            cut = cut_in_list(n, bin, !count, need, above);
+            if (!count || !again) break;
             clear();                            // p of the tokens up to the cut
             each_listed(n, [&](float x, int i) {
                 if (place_of(x, i) >= cut) atomicAdd(&sm.mass[w.bin(x)], w(x));
@@ -610,15 +631,6 @@ struct Draw {
             bin = sm.bin;
             above = sm.above;
         }
-        if (cut == 0) {                         // many in the cut's bin: all of the list in order
-            sort_list<NT>(sm.list, n);
-            cut = cut_in_list(n, !l.by_count, l.by_count ? (u64)l.k : l.need, 0);
-            if (again) {
-                u64 mass = 0;
-                each_listed(n, [&](float x, int i) { mass += place_of(x, i) >= cut ? w(x) : 0; });
-                cut = cut_in_list(n, true, share(p, block_all(mass, sm, Add{})), 0);
-            }
-        }
         from_listed(n, with_floor(cut));
     }
 
@@ -628,18 +640,19 @@ struct Draw {
         const u64 floor = with_floor(kNoCut);
         u64 cut = kNoCut;
         Plan l{};
+        bool by_count = k > 0, first = true;
 #pragma unroll 1
-        for (bool first = true; k > 0 || nucleus; first = false) {
+        while (by_count || nucleus) {
             clear();
-            fill(0, row.cols, first, nucleus, cut);
-            l = plan(first ? k : 0, p, first && k > 0);
-            if (!l.cut) break;
+            fill(0, row.cols, first, !by_count, cut);
+            l = plan(k, p, by_count);
             l.take &= first;
-            if (l.by_count && nucleus && !l.take) {             // a cut by number, then p of the tokens up to it
+            if (!by_count || (l.cut && (l.take || !nucleus))) break;
+            if (l.cut) {                        // a cut by number, then p of the tokens up to it
                 cut = cut_of(l, sweep<false>(0, row.cols, l, floor));
-                continue;
+                first = false;
             }
-            break;
+            by_count = false;
         }
         if (l.take) {
             const int n = (int)sweep<false>(0, row.cols, l, floor);
@@ -790,7 +803,8 @@ template <class T>
 __device__ __forceinline__ Plan plan_of(const Part<T>& q, const Draw<T, NS>& d, const Ask& ask) {
     for (int i = threadIdx.x; i < 2 * NS; i += NS) d.sm.count[i] = q.ws.count[i], d.sm.mass[i] = q.ws.mass[i];
     __syncthreads();
-    return d.plan(ask.k, ask.p, ask.k > 0);
+    const Plan l = d.plan(ask.k, ask.p, ask.k > 0);
+    return ask.k && !l.cut ? d.plan(0, ask.p, false) : l;
 }
 // A top-k of many tokens with a nucleus among them: one workgroup does such a row.
 __device__ __forceinline__ bool hard(const Plan& l, const Ask& ask) { return l.by_count && !l.take && ask.p < 1.f; }
