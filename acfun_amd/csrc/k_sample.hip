@@ -201,10 +201,26 @@ struct Row {
     // f(x, i) B neighbours at once, the first one's index i.  (One copy of f for each: what runs
     // a few times is fetched as it runs.)
     static constexpr int B = 4;
-    template <class F>
+    template <int U, class F>
     __device__ __forceinline__ void fours(int i0, int i1, int t, int threads, F f) const {
         int i = i0 + t * V;
         const int step = threads * V;
+        if constexpr (U > 1)
+#pragma unroll 1
+            for (; i + (U - 1) * step + V <= i1; i += U * step) {
+                VT v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = *(const VT*)(x + i + u * step);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int g = 0; g < V; g += B) {
+                        float y[B];
+#pragma unroll
+                        for (int e = 0; e < B; ++e) y[e] = (float)v[u][g + e];
+                        f(y, i + u * step + g);
+                    }
+            }
         if (i >= i1) return;
         Some s = load(i);
 #pragma unroll 1
@@ -223,9 +239,9 @@ struct Row {
         }
     }
     // one by one
-    template <class F>
+    template <int U = 1, class F>
     __device__ __forceinline__ void each(int i0, int i1, int t, int threads, F f) const {
-        fours(i0, i1, t, threads, [&](const float (&x)[B], int i) {
+        fours<U>(i0, i1, t, threads, [&](const float (&x)[B], int i) {
 #pragma unroll
             for (int e = 0; e < B; ++e) f(x[e], i + e);
         });
@@ -261,7 +277,7 @@ struct Plan {
 
 template <class T, int NT>
 struct Draw {
-    static constexpr int kWaves = NT / 64, kBins = 2 * NT, kList = 2 * NT;
+    static constexpr int kWaves = NT / 64, kBins = 2 * NT, kList = 2 * NT, kLoads = NT == 1024 && sizeof(T) == 4 ? 2 : 1;
     const Row<T> row;
     const Weights w;
     Shared<NT>& sm;
@@ -453,7 +469,7 @@ struct Draw {
     __device__ __forceinline__ u64 kept_mass(int a, int b, u64 cut, int t, int threads) const {
         const Cut c(cut);
         u64 mass = 0;
-        row.fours(a, b, t, threads, [&](const float (&x)[4], int i) {
+        row.template fours<kLoads>(a, b, t, threads, [&](const float (&x)[4], int i) {
             u64 m[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) m[e] = w(x[e]);
@@ -548,7 +564,7 @@ struct Draw {
     // The histogram of the tokens i0 to i1 not below the cut.
     __device__ __forceinline__ void fill(int i0, int i1, bool count, bool mass, u64 cut) const {
         const Cut c(cut);
-        row.fours(i0, i1, threadIdx.x, NT, [&](const float (&x)[4], int i) {
+        row.template fours<kLoads>(i0, i1, threadIdx.x, NT, [&](const float (&x)[4], int i) {
             u64 m[4] = {};
             if (mass)
 #pragma unroll
@@ -575,7 +591,7 @@ struct Draw {
         const unsigned b0 = l.take ? 0 : l.bin, b1 = l.cut ? l.bin : (unsigned)kBins;
         const Cut c(floor);
         u64 mass = 0;
-        row.fours(a, b, lane, 64, [&](const float (&x)[4], int i) {
+        row.template fours<kLoads>(a, b, lane, 64, [&](const float (&x)[4], int i) {
             u64 m[4] = {};
             if constexpr (MASS)
 #pragma unroll
@@ -681,7 +697,7 @@ struct Draw {
 template <int NT, class T>
 __device__ __forceinline__ float largest_of(const Row<T>& row, int i0, int i1, Shared<NT>& sm) {
     float top = -__builtin_inff();
-    row.each(i0, i1, threadIdx.x, NT, [&](float x, int) { top = __builtin_fmaxf(top, x); });
+    row.template each<NT == 1024 ? 8 : 1>(i0, i1, threadIdx.x, NT, [&](float x, int) { top = __builtin_fmaxf(top, x); });
     return block_all(top, sm, [](float p, float q) { return __builtin_fmaxf(p, q); });
 }
 // What a row asks for.
