@@ -76,13 +76,15 @@ void staged(const char* who, F f) {
     });
 }
 
+constexpr const char* kQ8Long = "K is more than 131072: sums of products could pass 32 bits";
+
 // A product of Q8 operands, or (rows) a layer on float rows.
 int q8_product(const char* who, const Q8Product& p, int type, bool rows, void* stream) {
     Checks c{who};
     c.type(type).need(p.act >= 0 && p.act <= ACFUN_GELU_TANH, "act is not 0 or one of ACFUN_RELU to ACFUN_GELU_TANH");
     if (!c.need(p.M >= 0 && p.N >= 0 && p.K >= 0, "a size is negative").ok) return -1;
     if (p.M == 0 || p.N == 0) return 0;
-    c.need(p.K <= kQ8MaxK, "K is more than 131072: sums of products could pass 32 bits");
+    c.need(p.K <= kQ8MaxK, kQ8Long);
     const int mats = p.gated ? 2 : 1;
     const size_t n = (size_t)p.M * p.N * type_size(type);
     if (p.K > 0) {
@@ -229,6 +231,7 @@ int acfun_dev_quantize_q8(const void* x, int type, int rows, int K, int trans, i
     Checks c{"acfun_dev_quantize_q8"};
     if (!c.type(type).need(rows >= 0 && K >= 0, "a size is negative").ok) return -1;
     if (rows == 0 || K == 0) return 0;
+    c.need(K <= kQ8MaxK, kQ8Long);
     if (!c.tensor(x, type, "x is NULL").held(codes, scales).ok) return -1;
     const size_t n = (size_t)rows * K * type_size(type);
     c.apart(codes, q8_code_bytes(rows, K), x, n).apart(scales, q8_scale_bytes(rows), x, n);
@@ -242,6 +245,7 @@ int acfun_dev_dequantize_q8(const int8_t* codes, const float* scales, int rows, 
     Checks c{"acfun_dev_dequantize_q8"};
     if (!c.type(type).need(rows >= 0 && K >= 0, "a size is negative").ok) return -1;
     if (rows == 0 || K == 0) return 0;
+    c.need(K <= kQ8MaxK, kQ8Long);
     if (!c.tensor(x, type, "x is NULL").held(codes, scales).ok) return -1;
     const size_t n = (size_t)rows * K * type_size(type);
     if (!c.apart(x, n, codes, q8_code_bytes(rows, K)).apart(x, n, scales, q8_scale_bytes(rows)).ok) return -1;

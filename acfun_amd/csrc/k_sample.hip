@@ -33,8 +33,8 @@ __device__ __forceinline__ float value_of(unsigned key) {
 // A token's place in the order, the first the largest.
 __device__ __forceinline__ u64 place_of(float x, int i) { return (u64)key_of(x) << 32 | (unsigned)~i; }
 
-// A cut below all that can be drawn: the place of -infinity.
-constexpr u64 kNoCut = (u64)0x007fffff << 32 | 0xffffffffu;
+// A cut below all that can be drawn: any index with the lowest finite value.
+constexpr u64 kNoCut = (u64)0x00800000 << 32;
 // Whether a token is not below a cut.
 struct Cut {
     float x;
@@ -101,7 +101,7 @@ struct Weights {
     // from 0 for the largest value up; `bins`: no weight (so for a NaN or -infinity)
     __device__ __forceinline__ unsigned bin(float x) const {
         const float b = __builtin_fmaf(x, -0.5f, half_top) * per_2x;    // (top - x may pass fp32)
-        return x <= top && !(b >= (float)bins) ? (unsigned)b : bins;    // (both infinite: bin 0)
+        return b < (float)bins ? (unsigned)b : x == top ? 0u : bins;    // (both infinite, b is none: 0)
     }
     // The least key whose weight is m or more, in (0, 1]: 64 candidates at once.
     __device__ __forceinline__ unsigned least_key(double m) const {

@@ -314,7 +314,7 @@ void acfun_fc_mxfp4(const float* input, int N, int Cin, const uint8_t* weight, c
  * have a scale for each output channel, activations one for each token.
  *
  * An operand of `rows` rows is two arrays, each aligned to 16 bytes (rows padded to 16,
- * K to 64, with zeros):
+ * K, of at most 131072, to 64, with zeros):
  *   codes   tiles of 16 rows x 64 k, row tiles outermost, 1024 bytes each: byte
  *           (16 j + r) * 16 + i of a tile holds k = 16 j + i of row r;
  *   scales  one fp32 for each row.
@@ -338,9 +338,9 @@ int acfun_dev_dequantize_q8(const int8_t* codes, const float* scales, int rows, 
 #define ACFUN_GELU_TANH 4  /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
 
 /* C[M,N] = act(A * B^T + bias[n]) (bias NULL = none), A an operand of M rows, B of N rows;
- * C of `type`.  Sums are exact (32-bit integers, for which K is at most 131072) and
- * become (sum * A's scale) * B's scale in fp32, whatever the sizes: a row's result does
- * not depend on the other rows of its call.  K = 0 gives act(bias). */
+ * C of `type`.  Sums are exact (32-bit integers, whose range bounds K) and become
+ * (sum * A's scale) * B's scale in fp32, whatever the sizes: a row's result does not
+ * depend on the other rows of its call.  K = 0 gives act(bias). */
 int acfun_dev_gemm_q8(int M, int N, int K, const int8_t* A, const float* a_scales, const int8_t* B,
                       const float* b_scales, void* C, int type, const float* bias, int act, void* stream);
 /* A fully connected layer with weights held in Q8 (an operand of Cout rows): input

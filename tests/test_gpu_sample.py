@@ -152,6 +152,27 @@ def test_settings_at_their_ends(gpu, rng):
         _check(gpu, x, "f32", u, k=np.full(12, k))
 
 
+@pytest.mark.parametrize("T", [float("inf"), 1e38, 3.0, 1e-40])
+@pytest.mark.parametrize("cols", [5, 5000, 40000])
+def test_masked_at_any_temperature(gpu, rng, cols, T):
+    """Most tokens ruled out, the first among them, or not a number; finite ones over all of
+    fp32's range."""
+    x = _logits(rng, 8, cols, "f32")
+    x[::2] *= 1e38
+    with np.errstate(over="ignore"):
+        x = x.astype(np.float32).astype(np.float64)
+    for r in range(8):
+        x[r, rng.integers(0, cols, 3 * cols)] = [-np.inf, np.nan][r % 2]
+        x[r, cols // 2 + r % 2] = 2.0
+    x[:, 0] = -np.inf
+    u, full = rng.random(8), lambda v: np.full(8, v)  # noqa: E731
+    _check(gpu, x, "f32", u, T=full(T))
+    _check(gpu, x, "f32", u, T=full(T), k=full(2))
+    _check(gpu, x, "f32", u, T=full(T), k=full(cols - 1), p=full(0.9))
+    _check(gpu, x, "f32", u, T=full(T), p=full(0.5), m=full(0.1))
+    _check(gpu, x, "f32", full(0.0), T=full(T), p=full(0.5), m=full(0.1))
+
+
 @pytest.mark.parametrize("rows", [1, 2, 17, 300, 1100])
 def test_rows_alone(gpu, rng, rows):
     """A row's token is the same in every batch."""

@@ -32,6 +32,7 @@ def test_quantize():
         _refused(f(t=-1), "type")
         _refused(f(r=-1), "negative")
         _refused(f(k=-5), "negative")
+        _refused(f(k=131073), "131072")
         for p in "xcs":
             _refused(f(**{p: None}), "NULL")
         _refused(f(c=Q[1] + 8), "aligned")
