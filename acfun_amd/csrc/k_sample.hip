@@ -12,6 +12,12 @@
 // even in x / T, 59 to a factor of e, so that most rows spread over many.  A top-k's
 // tokens, or a nucleus's, that are few are all taken out of the row, and the rest is done
 // with these.
+//
+// A row is read three to five times from the caches, and a few rows wait for what follows one
+// another: 64 x 32003 bf16 from a graph takes 7.5 us for the largest, 18.6 with a temperature,
+// 29 with top-k, 40 with a nucleus, 34 with all; 64 x 1000 fp32 3.7, 5.9, 10, 12 and 16.
+// Many rows are bound by the exponential in 64 bits, 18 instructions of each weight, and the
+// histogram's: 512 x 131072 fp32, all settings mixed, 247 us, of which memory needs 55.
 #include <type_traits>
 
 #include "q8.hpp"
@@ -29,6 +35,39 @@ __device__ __forceinline__ unsigned key_of(float x) {
 }
 __device__ __forceinline__ float value_of(unsigned key) {
     return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
+// What all lanes have, in scalar registers.
+__device__ __forceinline__ unsigned same(unsigned v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ u64 same(u64 v) { return (u64)same((unsigned)(v >> 32)) << 32 | same((unsigned)v); }
+// A value of 4 or 8 bytes from another lane: by DPP (lanes without a source, and rows not in
+// ROWS, get 0), and a lane's for all.  Sums by DPP take a third of the time that they do
+// through LDS.
+template <int CTRL, int ROWS = 15, class V>
+__device__ __forceinline__ V dpp(V v) {
+    if constexpr (sizeof(V) == 8)
+        return (V)dpp<CTRL, ROWS>((unsigned)((u64)v >> 32)) << 32 | dpp<CTRL, ROWS>((unsigned)v);
+    else
+        return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 15, false));
+}
+template <class V>
+__device__ __forceinline__ V from_lane(V v, int lane) {
+    if constexpr (sizeof(V) == 8)
+        return (V)from_lane((unsigned)((u64)v >> 32), lane) << 32 | from_lane((unsigned)v, lane);
+    else
+        return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+// The lanes of a set that are before this one.
+__device__ __forceinline__ unsigned before_in(u64 lanes) {
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0));
+}
+// f over the first N lanes of each 16, in these lanes.
+template <int N, class V, class F>
+__device__ __forceinline__ V row_all(V v, F f) {
+    if constexpr (N > 1) v = f(v, dpp<0xb1>(v));            // lane ^ 1
+    if constexpr (N > 2) v = f(v, dpp<0x4e>(v));            // lane ^ 2
+    if constexpr (N > 4) v = f(v, dpp<0x141>(v));           // 7 - lane, of each 8
+    if constexpr (N > 8) v = f(v, dpp<0x140>(v));           // 15 - lane
+    return v;
 }
 // A token's place in the order, the first the largest.
 __device__ __forceinline__ u64 place_of(float x, int i) { return (u64)key_of(x) << 32 | (unsigned)~i; }
@@ -76,7 +115,7 @@ struct Weights {
         half_top = 0.5f * top;
         max = inf ? 0x1.fffffep+127 : (double)top;
         c = inf ? 1. : 0x1.71547652b82fep+0 / (double)T;
-        least = -1000. / c;                     // (-infinity where T is infinite)
+        least = inf ? -1000. : -1000. * 0x1.62e42fefa39efp-1 * (double)T;   // -1000 / c
         per_2x = __builtin_fminf((float)n * (float)(0x1.715476p+0 / 25.) / T, 1e30f);
         bins = (unsigned)n;
         frac = f;
@@ -110,8 +149,8 @@ struct Weights {
             const unsigned lane = threadIdx.x & 63, k = lo + (unsigned)((u64)(hi - lo) * lane >> 6);
             const u64 past = __ballot(real(value_of(k)) >= m);
             const int s = past ? __ffsll(past) - 1 : 64;
-            if (s < 64) hi = __shfl(k, s);
-            if (s > 0) lo = __shfl(k, s - 1) + 1;
+            if (s < 64) hi = from_lane(k, s);
+            if (s > 0) lo = from_lane(k, s - 1) + 1;
         }
         return hi;
     }
@@ -138,9 +177,8 @@ struct Add { template <class V> __device__ V operator()(V a, V b) const { return
 
 template <class V, class F>
 __device__ __forceinline__ V wave_all(V v, F f) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v = f(v, (V)__shfl_xor(v, d));
-    return v;
+    v = row_all<16>(v, f);
+    return f(f(from_lane(v, 0), from_lane(v, 16)), f(from_lane(v, 32), from_lane(v, 48)));
 }
 template <int NT, class V, class F>
 __device__ __forceinline__ V block_all(V v, Shared<NT>& sm, F f) {
@@ -149,19 +187,17 @@ __device__ __forceinline__ V block_all(V v, Shared<NT>& sm, F f) {
     if ((threadIdx.x & 63) == 0) sm.part[threadIdx.x >> 6] = __builtin_bit_cast(U, v);
     __syncthreads();
     v = __builtin_bit_cast(V, (U)sm.part[threadIdx.x % (NT / 64)]);
-#pragma unroll
-    for (int d = 1; d < NT / 64; d *= 2) v = f(v, (V)__shfl_xor(v, d));
     __syncthreads();
-    return v;
+    return from_lane(row_all<NT / 64>(v, f), 0);
 }
 // The sum over the lanes up to and with this one, of the wave and of the block.
 __device__ __forceinline__ u64 wave_upto(u64 v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const u64 o = __shfl_up(v, d);
-        if ((int)(threadIdx.x & 63) >= d) v += o;
-    }
-    return v;
+    v += dpp<0x111>(v);                                     // lane - 1, 2, 4, 8 of a row of 16
+    v += dpp<0x112>(v);
+    v += dpp<0x114>(v);
+    v += dpp<0x118>(v);
+    v += dpp<0x142, 10>(v);                                 // rows 1 and 3: the row before's last lane
+    return v + dpp<0x143, 12>(v);                           // rows 2 and 3: lane 31
 }
 template <int NT>
 __device__ __forceinline__ u64 block_upto(u64 v, Shared<NT>& sm, u64& total) {
@@ -170,9 +206,9 @@ __device__ __forceinline__ u64 block_upto(u64 v, Shared<NT>& sm, u64& total) {
     if ((threadIdx.x & 63) == 63) sm.part[threadIdx.x >> 6] = v;
     __syncthreads();
     const u64 waves = wave_upto((int)(threadIdx.x & 63) < W ? sm.part[threadIdx.x % W] : 0);
-    total = __shfl(waves, W - 1);
-    const int w = threadIdx.x >> 6;
-    const u64 before = __shfl(waves, w ? w - 1 : 0);
+    total = from_lane(waves, W - 1);
+    const int w = (int)same(threadIdx.x >> 6);
+    const u64 before = from_lane(waves, w ? w - 1 : 0);
     __syncthreads();
     return w ? v + before : v;
 }
@@ -270,9 +306,9 @@ __device__ __forceinline__ bool find_bin(const V* bins, u64 need, Shared<NT>& sm
 // the next cut lies in, and whether the tokens up to it are few enough to take them all.
 struct Plan {
     bool by_count, cut, take;                   // cut: there is one
-    int k;
     unsigned bin;
-    u64 need, above, mass;                      // mass: of all tokens (not by_count)
+    u64 need, above;
+    unsigned lo = ~0u, hi = 0;                  // the bins of the list
 };
 
 template <class T, int NT>
@@ -289,7 +325,7 @@ struct Draw {
     __device__ __forceinline__ u64 with_floor(u64 cut) const {
         if (!(m > 0.f)) return cut;
         const u64 floor = (u64)w.least_key(m < 1.f ? (double)m : 1.) << 32;
-        return floor > cut ? floor : cut;
+        return same(floor > cut ? floor : cut);
     }
     template <class F>
     __device__ __forceinline__ void all(F f) const { row.each(0, row.cols, threadIdx.x, NT, f); }
@@ -322,8 +358,8 @@ struct Draw {
             __syncthreads();
             if constexpr (MASS) find_bin(sm.mass, need - before, sm);
             else find_bin(sm.count, need - before, sm);
-            prefix = prefix << width | ((1u << width) - 1 - sm.bin);
-            before += sm.above;
+            prefix = prefix << width | ((1u << width) - 1 - same(sm.bin));
+            before += same(sm.above);
             __syncthreads();
             if (shift == 0) return prefix;
             shift = shift > D ? shift - D : 0;
@@ -384,7 +420,7 @@ struct Draw {
             if (before < need && need <= before + sm.some_mass[t]) sm.above = mine;
         }
         __syncthreads();
-        const u64 c = sm.above;
+        const u64 c = same(sm.above);
         __syncthreads();
         return c;
     }
@@ -500,10 +536,10 @@ struct Draw {
                 __syncthreads();
             }
             const u64 upto = wave_upto(lane < kWaves ? sm.part[lane % kWaves] : 0);
-            if (!total) total = __shfl(upto, kWaves - 1), target = target_of(total);
+            if (!total) total = from_lane(upto, kWaves - 1), target = target_of(total);
             const u64 past = __ballot(lane < kWaves && before + upto > target);
             const int s = past ? __ffsll(past) - 1 : kWaves - 1;
-            before += s ? __shfl(upto, s - 1) : 0;
+            before += s ? from_lane(upto, s - 1) : 0;
             __syncthreads();
             i0 += s * per;
             i1 = i0 + per < i1 ? i0 + per : i1;
@@ -542,53 +578,85 @@ struct Draw {
 
     __device__ __forceinline__ Plan plan(int k, float p, bool by_count) const {
         const int t = threadIdx.x;
-        Plan l{by_count, true, false, k, 0, (u64)k, 0, 0};
+        Plan l{by_count, true, false, 0, (u64)k, 0};
         if (by_count) {                         // (fewer tokens than k that weigh anything: no limit)
             l.cut = find_bin(sm.count, l.need, sm);
         } else if (p < 1.f) {
-            l.mass = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{});
-            l.need = share(p, l.mass);
+            l.need = same(share(p, block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{})));
             find_bin(sm.mass, l.need, sm);
         } else {
             l.cut = false;
         }
-        l.bin = sm.bin;
-        l.above = sm.above;
+        l.bin = same(sm.bin);
+        l.above = same(sm.above);
         __syncthreads();
         if (!l.cut) return l;
         const unsigned few =
             (2 * t <= (int)l.bin ? sm.count[2 * t] : 0) + (2 * t + 1 <= (int)l.bin ? sm.count[2 * t + 1] : 0);
-        l.take = block_all(few, sm, Add{}) <= (unsigned)kList;
+        l.take = same(block_all(few, sm, Add{})) <= (unsigned)kList;
+        l.lo = l.take ? 0 : l.bin;
+        l.hi = l.bin;
         return l;
     }
-    // The histogram of the tokens i0 to i1 not below the cut.
-    __device__ __forceinline__ void fill(int i0, int i1, bool count, bool mass, u64 cut) const {
-        const Cut c(cut);
-        row.template fours<kLoads>(i0, i1, threadIdx.x, NT, [&](const float (&x)[4], int i) {
-            u64 m[4] = {};
-            if (mass)
+    // The plan of a nucleus by the bins' numbers alone, with the weight in a bin's middle: the
+    // next bins on both sides are listed too while there is room, and the exact sums of the pass
+    // that lists them say whether the cut is there.
+    __device__ __forceinline__ Plan guess(float p) const {
+        const int t = threadIdx.x;
+#pragma unroll
+        for (int b = 2 * t; b < 2 * t + 2; ++b)
+            sm.mass[b] = (u64)((double)sm.count[b] *
+                               (double)__builtin_amdgcn_exp2f((float)w.frac - ((float)b + 0.5f) * (50.f / kBins)));
+        Plan l = plan(0, p, false);
+        l.hi = l.bin + 1 < (unsigned)kBins ? l.bin + 1 : l.bin;
+        unsigned wide = l.bin ? l.bin - 1 : 0;
+        u64 upto = 0;
+        for (int b = 2 * t; b < 2 * t + 2; ++b)
+            if (b <= (int)l.hi) upto += sm.count[b] + (b >= (int)wide ? (u64)sm.count[b] << 32 : 0);
+        upto = same(block_all(upto, sm, Add{}));
+        l.take = (unsigned)upto <= (unsigned)kList;
+        const bool fits = (unsigned)(upto >> 32) <= (unsigned)kList;
+        l.lo = l.take ? 0 : fits ? wide : l.bin;
+        l.hi = fits ? l.hi : l.bin;
+        return l;
+    }
+    // The histogram of the tokens i0 to i1: of their number, or (`mass`) of both the number and
+    // the mass of those not below the cut.
+    __device__ __forceinline__ void fill(int i0, int i1, bool mass, u64 cut) const {
+        if (!mass)
+            row.template fours<kLoads>(i0, i1, threadIdx.x, NT, [&](const float (&x)[4], int) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (const unsigned b = w.bin(x[e]); b < (unsigned)kBins) atomicAdd(&sm.count[b], 1u);
+            });
+        else {
+            const Cut c(cut);
+            row.template fours<kLoads>(i0, i1, threadIdx.x, NT, [&](const float (&x)[4], int i) {
+                u64 m[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) m[e] = w(x[e]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned b = w.bin(x[e]);
-                if (b >= (unsigned)kBins || !c.keeps(x[e], i + e)) continue;
-                if (count) atomicAdd(&sm.count[b], 1u);
-                if (mass) atomicAdd(&sm.mass[b], m[e]);
-            }
-        });
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned b = w.bin(x[e]);
+                    if (b >= (unsigned)kBins || !c.keeps(x[e], i + e)) continue;
+                    atomicAdd(&sm.count[b], 1u);
+                    atomicAdd(&sm.mass[b], m[e]);
+                }
+            });
+        }
         __syncthreads();
     }
-    // One pass over the tokens i0 to i1, a run to each wave.  To the list: those of the bins up
-    // to l's (l.take), or of that alone; their number is the result.  To sm.part (MASS): the
-    // masses of the runs' tokens before that bin, or of all (not l.cut), without those below `floor`.
+    // One pass over the tokens i0 to i1, a run to each wave.  To the list: those of l's bins;
+    // their number is the result.  To sm.part (MASS): the masses of the runs' tokens before these
+    // bins, or of all (no bins), without those below `floor`.  To a thread's sums: of its tokens
+    // in the bins, and of all.
+    struct Sums { u64 listed = 0, total = 0; };
     template <bool MASS>
-    __device__ __forceinline__ unsigned sweep(int i0, int i1, const Plan& l, u64 floor) const {
+    __device__ __forceinline__ unsigned sweep(int i0, int i1, const Plan& l, u64 floor, Sums* sums = nullptr) const {
         if (threadIdx.x == 0) sm.n = 0;
         __syncthreads();
         const int per = run_of(i0, i1), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         const int a = i0 + wave * per < i1 ? i0 + wave * per : i1, b = a + per < i1 ? a + per : i1;
-        const unsigned b0 = l.take ? 0 : l.bin, b1 = l.cut ? l.bin : (unsigned)kBins;
         const Cut c(floor);
         u64 mass = 0;
         row.template fours<kLoads>(a, b, lane, 64, [&](const float (&x)[4], int i) {
@@ -596,13 +664,29 @@ struct Draw {
             if constexpr (MASS)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) m[e] = w(x[e]);
+            bool in[4];
+            u64 has[4];
+            unsigned hits = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const unsigned at = w.bin(x[e]);
-                if (MASS) mass += at < b1 && c.keeps(x[e], i + e) ? m[e] : 0;
-                if (at < b0 || at > b1 || !l.cut) continue;
-                const unsigned n = atomicAdd(&sm.n, 1u);
-                if (n < (unsigned)kList) sm.list[n] = place_of(x[e], i + e);
+                if (MASS) mass += at < l.lo && c.keeps(x[e], i + e) ? m[e] : 0;
+                if (MASS && sums) sums->total += m[e];
+                in[e] = at >= l.lo && at <= l.hi;
+                if (MASS && sums) sums->listed += in[e] ? m[e] : 0;
+                has[e] = __ballot(in[e]);
+                hits += __popcll(has[e]);
+            }
+            if (!hits) return;
+            // one atomic for the wave's four
+            unsigned n = 0;
+            if (!before_in(__ballot(1))) n = atomicAdd(&sm.n, hits);
+            n = same(n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned to = n + before_in(has[e]);
+                if (in[e] && to < (unsigned)kList) sm.list[to] = place_of(x[e], i + e);
+                n += __popcll(has[e]);
             }
         });
         if constexpr (MASS) {
@@ -610,7 +694,7 @@ struct Draw {
             if (lane == 0) sm.part[wave] = mass;
         }
         __syncthreads();
-        const unsigned n = sm.n;
+        const unsigned n = same(sm.n);
         __syncthreads();
         return n;
     }
@@ -656,38 +740,61 @@ struct Draw {
         const u64 floor = with_floor(kNoCut);
         u64 cut = kNoCut;
         Plan l{};
-        bool by_count = k > 0, first = true;
+        bool by_count = k > 0, exact = false, runs = false;
 #pragma unroll 1
-        while (by_count || nucleus) {
-            clear();
-            fill(0, row.cols, first, !by_count, cut);
-            l = plan(k, p, by_count);
-            l.take &= first;
-            if (!by_count || (l.cut && (l.take || !nucleus))) break;
-            if (l.cut) {                        // a cut by number, then p of the tokens up to it
-                cut = cut_of(l, sweep<false>(0, row.cols, l, floor));
-                first = false;
+        for (;;) {
+            if (!by_count && !nucleus) {
+                cut = floor;
+                break;
             }
+            clear();
+            fill(0, row.cols, !by_count && exact, cut);
+            l = by_count || exact ? plan(k, p, by_count) : guess(p);
+            if (exact) l.take = false, l.lo = l.bin;    // (a cut by number counts, the list would not know it)
             by_count = false;
-        }
-        if (l.take) {
-            const int n = (int)sweep<false>(0, row.cols, l, floor);
-            from_list(n, l, p);
-            return;
-        }
-        bool runs = false;
-        if (l.cut) {
-            const unsigned n = sweep<true>(0, row.cols, l, floor);
-            runs = n <= (unsigned)kList;
-            const u64 mine = sm.part[threadIdx.x % kWaves];     // (what finds the cut uses them)
+            if (!l.cut) continue;               // no limit
+            const bool listed_only = l.by_count && (l.take || nucleus);
+            Sums sums;
+            const unsigned n = listed_only ? sweep<false>(0, row.cols, l, floor) : sweep<true>(0, row.cols, l, floor, &sums);
+            const u64 mine = sm.part[threadIdx.x % kWaves];     // (what follows uses them)
             __syncthreads();
-            cut = cut_of(l, n);
+            bool past = false;                  // min_p ends before the list
+            if (!l.by_count && !exact) {
+                const u64 before = from_lane(row_all<kWaves>(mine, Add{}), 0);
+                const u64 listed = same(block_all(sums.listed, sm, Add{}));
+                l.need = same(share(p, block_all(sums.total, sm, Add{})));
+                past = w.bin(value_of(floor >> 32)) < l.lo;
+                if (before >= l.need || (!past && before + listed < l.need)) {
+                    exact = true;
+                    continue;
+                }
+                l.bin = l.lo;
+                l.above = before;
+                if (l.lo < l.hi && !past) {     // the list's bin with the cut
+                    clear();
+                    each_listed((int)n, [&](float x, int i) { atomicAdd(&sm.mass[w.bin(x)], w(x)); });
+                    __syncthreads();
+                    find_bin(sm.mass, l.need - before, sm);
+                    l.bin = same(sm.bin);
+                    l.above += same(sm.above);
+                    __syncthreads();
+                }
+            }
+            if (l.take) {
+                from_list((int)n, l, p);
+                return;
+            }
+            cut = past ? floor : cut_of(l, n);
+            if (listed_only) {                  // a cut by number, then p of the tokens up to it
+                exact = true;
+                continue;
+            }
             cut = cut > floor ? cut : floor;
+            runs = n <= (unsigned)kList;
             if (threadIdx.x < kWaves) sm.part[threadIdx.x] = mine;
             __syncthreads();
             if (runs) add_list((int)n, cut, 0, run_of(0, row.cols), sm.part);
-        } else {
-            cut = floor;
+            break;
         }
         from_row(0, row.cols, cut, 0, 0, runs);
     }
@@ -806,7 +913,7 @@ __global__ __launch_bounds__(NS) void k_sample_bins(Split p) {
     if (plain(top, ask)) return;
     const auto d = q.draw(p, top, ask, sm);
     d.clear();
-    d.fill(q.i0, q.i1, true, ask.p < 1.f, kNoCut);
+    d.fill(q.i0, q.i1, ask.p < 1.f, kNoCut);
 #pragma unroll
     for (int i = threadIdx.x; i < 2 * NS; i += NS) {
         if (sm.count[i]) atomicAdd(&q.ws.count[i], sm.count[i]);
@@ -892,9 +999,9 @@ __global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
     }
     const int lane = threadIdx.x & 63;
     const u64 upto = wave_upto(lane < p.parts ? kept[lane] : 0);
-    const u64 total = __shfl(upto, 63), target = d.target_of(total), past = __ballot(upto > target);
+    const u64 total = from_lane(upto, 63), target = d.target_of(total), past = __ballot(upto > target);
     const int s = __ffsll(past) - 1;
-    const u64 before = s ? __shfl(upto, s - 1) : 0;
+    const u64 before = s ? from_lane(upto, s - 1) : 0;
     const int i0 = s * p.per;
     d.from_row(i0, i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols, cut, before, total, false);
 }
