@@ -56,6 +56,7 @@ __device__ __forceinline__ V from_lane(V v, int lane) {
     else
         return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
+__device__ __forceinline__ u64 lanes_of(bool b) { return __builtin_amdgcn_ballot_w64(b); }
 // The lanes of a set that are before this one.
 __device__ __forceinline__ unsigned before_in(u64 lanes) {
     return __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0));
@@ -79,7 +80,7 @@ struct Cut {
     float x;
     unsigned i;
     __device__ __forceinline__ explicit Cut(u64 place) : x(value_of(place >> 32)), i(~(unsigned)place) {}
-    __device__ __forceinline__ bool keeps(float v, int at) const { return v > x || (v == x && (unsigned)at <= i); }
+    __device__ __forceinline__ bool keeps(float v, int at) const { return (v > x) | ((v == x) & ((unsigned)at <= i)); }
 };
 
 // 2^f, |f| <= 1/2, by the polynomial through it at nine Chebyshev points, off by 1.1e-12 of the
@@ -140,14 +141,15 @@ struct Weights {
     // from 0 for the largest value up; `bins`: no weight (so for a NaN or -infinity)
     __device__ __forceinline__ unsigned bin(float x) const {
         const float b = __builtin_fmaf(x, -0.5f, half_top) * per_2x;    // (top - x may pass fp32)
-        return b < (float)bins ? (unsigned)b : x == top ? 0u : bins;    // (both infinite, b is none: 0)
+        const unsigned at = (unsigned)__builtin_fminf(b, (float)bins);
+        return x == top ? 0u : at;                                      // (both infinite, b is none)
     }
     // The least key whose weight is m or more, in (0, 1]: 64 candidates at once.
     __device__ __forceinline__ unsigned least_key(double m) const {
         unsigned lo = key_of(-0x1.fffffep+127f), hi = key_of(top);
         while (lo < hi) {
             const unsigned lane = threadIdx.x & 63, k = lo + (unsigned)((u64)(hi - lo) * lane >> 6);
-            const u64 past = __ballot(real(value_of(k)) >= m);
+            const u64 past = lanes_of(real(value_of(k)) >= m);
             const int s = past ? __ffsll(past) - 1 : 64;
             if (s < 64) hi = from_lane(k, s);
             if (s > 0) lo = from_lane(k, s - 1) + 1;
@@ -537,7 +539,7 @@ struct Draw {
             }
             const u64 upto = wave_upto(lane < kWaves ? sm.part[lane % kWaves] : 0);
             if (!total) total = from_lane(upto, kWaves - 1), target = target_of(total);
-            const u64 past = __ballot(lane < kWaves && before + upto > target);
+            const u64 past = lanes_of(lane < kWaves && before + upto > target);
             const int s = past ? __ffsll(past) - 1 : kWaves - 1;
             before += s ? from_lane(upto, s - 1) : 0;
             __syncthreads();
@@ -670,17 +672,17 @@ struct Draw {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const unsigned at = w.bin(x[e]);
-                if (MASS) mass += at < l.lo && c.keeps(x[e], i + e) ? m[e] : 0;
+                if (MASS) mass += (at < l.lo) & c.keeps(x[e], i + e) ? m[e] : 0;
                 if (MASS && sums) sums->total += m[e];
-                in[e] = at >= l.lo && at <= l.hi;
+                in[e] = (at >= l.lo) & (at <= l.hi);
                 if (MASS && sums) sums->listed += in[e] ? m[e] : 0;
-                has[e] = __ballot(in[e]);
+                has[e] = lanes_of(in[e]);
                 hits += __popcll(has[e]);
             }
             if (!hits) return;
             // one atomic for the wave's four
             unsigned n = 0;
-            if (!before_in(__ballot(1))) n = atomicAdd(&sm.n, hits);
+            if (!before_in(lanes_of(true))) n = atomicAdd(&sm.n, hits);
             n = same(n);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -882,7 +884,7 @@ struct Part {
     // the first part that holds the row's largest
     __device__ __forceinline__ int of_top(const Split& p, float top) const {
         const int lane = threadIdx.x & 63;
-        return __ffsll(__ballot(lane < p.parts && ws.top[lane] == top)) - 1;
+        return __ffsll(lanes_of(lane < p.parts && ws.top[lane] == top)) - 1;
     }
     __device__ __forceinline__ Draw<T, NS> draw(const Split& p, float top, const Ask& ask, Shared<NS>& sm) const {
         return {row, Weights(top, ask.T, p.frac, 2 * NS), sm, p.a.token + r, p.a.prob ? p.a.prob + r : nullptr, ask.u,
@@ -999,7 +1001,7 @@ __global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
     }
     const int lane = threadIdx.x & 63;
     const u64 upto = wave_upto(lane < p.parts ? kept[lane] : 0);
-    const u64 total = from_lane(upto, 63), target = d.target_of(total), past = __ballot(upto > target);
+    const u64 total = from_lane(upto, 63), target = d.target_of(total), past = lanes_of(upto > target);
     const int s = __ffsll(past) - 1;
     const u64 before = s ? from_lane(upto, s - 1) : 0;
     const int i0 = s * p.per;
