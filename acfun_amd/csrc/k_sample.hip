@@ -601,25 +601,31 @@ struct Draw {
         return l;
     }
     // The plan of a nucleus by the bins' numbers alone, with the weight in a bin's middle: the
-    // next bins on both sides are listed too while there is room, and the exact sums of the pass
-    // that lists them say whether the cut is there.
+    // next bins on both sides are listed too while there is room (none, lo past hi: the bin alone
+    // has too many), and the exact sums of the pass that lists them say whether the cut is there.
     __device__ __forceinline__ Plan guess(float p) const {
         const int t = threadIdx.x;
 #pragma unroll
         for (int b = 2 * t; b < 2 * t + 2; ++b)
             sm.mass[b] = (u64)((double)sm.count[b] *
                                (double)__builtin_amdgcn_exp2f((float)w.frac - ((float)b + 0.5f) * (50.f / kBins)));
-        Plan l = plan(0, p, false);
+        find_bin(sm.mass, share(p, block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{})), sm);
+        Plan l{};
+        l.cut = true;
+        l.bin = same(sm.bin);
         l.hi = l.bin + 1 < (unsigned)kBins ? l.bin + 1 : l.bin;
-        unsigned wide = l.bin ? l.bin - 1 : 0;
+        // the tokens up to there, and those of the bin and the ones beside it
         u64 upto = 0;
         for (int b = 2 * t; b < 2 * t + 2; ++b)
-            if (b <= (int)l.hi) upto += sm.count[b] + (b >= (int)wide ? (u64)sm.count[b] << 32 : 0);
+            if (b <= (int)l.hi) upto += sm.count[b] + (b + 1 >= (int)l.bin ? (u64)sm.count[b] << 32 : 0);
         upto = same(block_all(upto, sm, Add{}));
         l.take = (unsigned)upto <= (unsigned)kList;
-        const bool fits = (unsigned)(upto >> 32) <= (unsigned)kList;
-        l.lo = l.take ? 0 : fits ? wide : l.bin;
-        l.hi = fits ? l.hi : l.bin;
+        l.lo = l.take ? 0 : l.bin ? l.bin - 1 : 0;
+        if (upto >> 32 > (u64)kList) {
+            l.hi = l.bin;
+            l.lo = same(sm.count[l.bin]) <= (unsigned)kList ? l.bin : ~0u;
+        }
+        __syncthreads();                        // (what follows may clear the numbers)
         return l;
     }
     // The histogram of the tokens i0 to i1: of their number, or (`mass`) of both the number and
@@ -650,16 +656,15 @@ struct Draw {
     }
     // One pass over the tokens i0 to i1, a run to each wave.  To the list: those of l's bins;
     // their number is the result.  To sm.part (MASS): the masses of the runs' tokens before these
-    // bins, or of all (no bins), without those below `floor`.  To a thread's sums: of its tokens
-    // in the bins, and of all.
-    struct Sums { u64 listed = 0, total = 0; };
+    // bins, or of all (no bins), without those below `floor`, a value's
+    // first place.  To `total`: the mass of a thread's tokens.
     template <bool MASS>
-    __device__ __forceinline__ unsigned sweep(int i0, int i1, const Plan& l, u64 floor, Sums* sums = nullptr) const {
+    __device__ __forceinline__ unsigned sweep(int i0, int i1, const Plan& l, u64 floor, u64* total = nullptr) const {
         if (threadIdx.x == 0) sm.n = 0;
         __syncthreads();
         const int per = run_of(i0, i1), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         const int a = i0 + wave * per < i1 ? i0 + wave * per : i1, b = a + per < i1 ? a + per : i1;
-        const Cut c(floor);
+        const float least = Cut(floor).x;
         u64 mass = 0;
         row.template fours<kLoads>(a, b, lane, 64, [&](const float (&x)[4], int i) {
             u64 m[4] = {};
@@ -672,10 +677,9 @@ struct Draw {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const unsigned at = w.bin(x[e]);
-                if (MASS) mass += (at < l.lo) & c.keeps(x[e], i + e) ? m[e] : 0;
-                if (MASS && sums) sums->total += m[e];
+                if (MASS) mass += (at < l.lo) & (x[e] >= least) ? m[e] : 0;
+                if (MASS && total) *total += m[e];
                 in[e] = (at >= l.lo) & (at <= l.hi);
-                if (MASS && sums) sums->listed += in[e] ? m[e] : 0;
                 has[e] = lanes_of(in[e]);
                 hits += __popcll(has[e]);
             }
@@ -752,35 +756,34 @@ struct Draw {
             clear();
             fill(0, row.cols, !by_count && exact, cut);
             l = by_count || exact ? plan(k, p, by_count) : guess(p);
+            if (l.lo > l.hi && l.cut) {         // no guess
+                exact = true;
+                continue;
+            }
             if (exact) l.take = false, l.lo = l.bin;    // (a cut by number counts, the list would not know it)
             by_count = false;
             if (!l.cut) continue;               // no limit
             const bool listed_only = l.by_count && (l.take || nucleus);
-            Sums sums;
-            const unsigned n = listed_only ? sweep<false>(0, row.cols, l, floor) : sweep<true>(0, row.cols, l, floor, &sums);
+            u64 total = 0;
+            const unsigned n = listed_only ? sweep<false>(0, row.cols, l, floor) : sweep<true>(0, row.cols, l, floor, &total);
             const u64 mine = sm.part[threadIdx.x % kWaves];     // (what follows uses them)
             __syncthreads();
             bool past = false;                  // min_p ends before the list
             if (!l.by_count && !exact) {
                 const u64 before = from_lane(row_all<kWaves>(mine, Add{}), 0);
-                const u64 listed = same(block_all(sums.listed, sm, Add{}));
-                l.need = same(share(p, block_all(sums.total, sm, Add{})));
+                l.need = same(share(p, block_all(total, sm, Add{})));
                 past = w.bin(value_of(floor >> 32)) < l.lo;
-                if (before >= l.need || (!past && before + listed < l.need)) {
-                    exact = true;
-                    continue;
-                }
-                l.bin = l.lo;
-                l.above = before;
-                if (l.lo < l.hi && !past) {     // the list's bin with the cut
+                exact = before >= l.need;
+                if (!exact && !past) {          // the list's bin with the cut
                     clear();
                     each_listed((int)n, [&](float x, int i) { atomicAdd(&sm.mass[w.bin(x)], w(x)); });
                     __syncthreads();
-                    find_bin(sm.mass, l.need - before, sm);
+                    exact = !find_bin(sm.mass, l.need - before, sm);
                     l.bin = same(sm.bin);
-                    l.above += same(sm.above);
+                    l.above = before + same(sm.above);
                     __syncthreads();
                 }
+                if (exact) continue;            // the guess was wrong
             }
             if (l.take) {
                 from_list((int)n, l, p);
