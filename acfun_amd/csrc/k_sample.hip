@@ -316,6 +316,7 @@ struct Plan {
 template <class T, int NT>
 struct Draw {
     static constexpr int kWaves = NT / 64, kBins = 2 * NT, kList = 2 * NT, kLoads = NT == 1024 && sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kFew = kLoads == 2 ? 4 : 1;    // loads where nothing else needs registers
     const Row<T> row;
     const Weights w;
     Shared<NT>& sm;
@@ -632,7 +633,7 @@ struct Draw {
     // the mass of those not below the cut.
     __device__ __forceinline__ void fill(int i0, int i1, bool mass, u64 cut) const {
         if (!mass)
-            row.template fours<kLoads>(i0, i1, threadIdx.x, NT, [&](const float (&x)[4], int) {
+            row.template fours<kFew>(i0, i1, threadIdx.x, NT, [&](const float (&x)[4], int) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (const unsigned b = w.bin(x[e]); b < (unsigned)kBins) atomicAdd(&sm.count[b], 1u);
@@ -666,7 +667,7 @@ struct Draw {
         const int a = i0 + wave * per < i1 ? i0 + wave * per : i1, b = a + per < i1 ? a + per : i1;
         const float least = Cut(floor).x;
         u64 mass = 0;
-        row.template fours<kLoads>(a, b, lane, 64, [&](const float (&x)[4], int i) {
+        row.template fours<MASS ? kLoads : kFew>(a, b, lane, 64, [&](const float (&x)[4], int i) {
             u64 m[4] = {};
             if constexpr (MASS)
 #pragma unroll
