@@ -14,10 +14,10 @@
 // with these.
 //
 // A row is read three to five times from the caches, and a few rows wait for what follows one
-// another: 64 x 32003 bf16 from a graph takes 7.5 us for the largest, 18.6 with a temperature,
-// 29 with top-k, 40 with a nucleus, 34 with all; 64 x 1000 fp32 3.7, 5.9, 10, 12 and 16.
-// Many rows are bound by the exponential in 64 bits, 18 instructions of each weight, and the
-// histogram's: 512 x 131072 fp32, all settings mixed, 247 us, of which memory needs 55.
+// another: 64 x 32003 bf16 takes 7.5 us for the largest, 15.7 with a temperature, 23 with a top-k,
+// 33 with a nucleus, 27 with all; 64 x 1000 fp32 3.7, 4.8, 8, 12 and 13.  Many rows are bound by the
+// instructions of a weight, the exponential in 64 bits above all: 512 x 131072 fp32 with a
+// nucleus takes 207 us, half of it the one pass with weights; the first, from memory, 46.
 #include <type_traits>
 
 #include "q8.hpp"

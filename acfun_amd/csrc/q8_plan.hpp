@@ -123,12 +123,13 @@ constexpr bool q8_rows_one(int M, int K) { return M <= 16 && M * (((long long)K 
 constexpr int kSampleMaxCols = 1 << 24, kSampleParts = 32;
 constexpr bool sample_fits(int rows) { return launch_fits(rows, 1024); }
 struct SamplePlan { int parts, per, threads; };
-// Parts from 24,576 columns on while a row has 1,024 columns for each row of the call.
-// Measured, us, mixed settings bf16 (in a graph, where it is one workgroup; from the host in
-// parts): 1 x 16384 21 and 24, 1 x 32768 26 and 24, 1 x 131072 59 and 25; 128 x 32768 43 and
-// 54, 128 x 65536 68 and 69, 128 x 131072 116 and 96, 256 x 131072 120 and 144.
+// Parts from 24,576 columns on while a row has 2,048 columns for each row of the call.
+// Measured, us, one workgroup (in a graph) and parts: mixed settings bf16 1 x 32768 18 and
+// 20, 1 x 131072 36 and 20, 16 x 65536 45 and 31, 64 x 131072 101 and 61; a nucleus fp32 1 x 32768
+// 28 and 23, 32 x 65536 47 and 41; all settings on fp32 1 x 32768 23 and 23, 32 x 65536 31 and
+// 37, 64 x 65536 32 and 41, 128 x 131072 52 and 68.
 inline SamplePlan sample_plan(int rows, int cols, int cus) {
-    if (cols < 24576 || (long long)rows * 1024 > cols)
+    if (cols < 24576 || (long long)rows * 2048 > cols)
         return {1, cols, cols <= 1024 ? 256 : cols <= 8192 ? 512 : 1024};
     int parts = (cols + 4095) / 4096;
     if (parts > kSampleParts) parts = kSampleParts;
