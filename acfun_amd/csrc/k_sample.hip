@@ -107,16 +107,17 @@ struct Weights {
     unsigned bins;
     int frac;
     Exp2 exp2;
-    // `bins` for the 50 powers of two that weigh; no infinity, whose product with 0 is none.  An
-    // infinite top is the largest fp32 here, and so is what equals it; other values are far
-    // from it at any temperature.
+    // `bins` for the 50 powers of two that weigh.  No infinities, whose differences and products
+    // are none: a temperature is 2^1000 at most, an infinite top is 2^128 (which it is not below,
+    // and finite values are far from at the temperature 1, as they are to be at any).
     __device__ __forceinline__ Weights(float largest, float T, int f, int n) {
         const bool inf = largest == __builtin_inff();
         top = largest;
         half_top = 0.5f * top;
-        max = inf ? 0x1.fffffep+127 : (double)top;
-        c = inf ? 1. : 0x1.71547652b82fep+0 / (double)T;
-        least = inf ? -1000. : -1000. * 0x1.62e42fefa39efp-1 * (double)T;   // -1000 / c
+        max = inf ? 0x1p128 : (double)top;
+        const double t = T < __builtin_inff() ? (double)T : 0x1p1000;
+        c = inf ? 1. : 0x1.71547652b82fep+0 / t;
+        least = inf ? -1000. : -1000. * 0x1.62e42fefa39efp-1 * t;           // -1000 / c
         per_2x = __builtin_fminf((float)n * (float)(0x1.715476p+0 / 25.) / T, 1e30f);
         bins = (unsigned)n;
         frac = f;
@@ -125,7 +126,7 @@ struct Weights {
     // below 1, added to the exponent; the result's steps again in such low bits.  2^-1000 and less
     // (-infinity, NaN) is 0 of them.
     __device__ __forceinline__ u64 operator()(float x) const {
-        const double d = __builtin_fmax((double)__builtin_fminf(x, 0x1.fffffep+127f) - max, least);
+        const double d = __builtin_fmin(__builtin_fmax((double)x - max, least), 0.);
         const double z = __builtin_fma(d, c, 0x1.8p52), f = __builtin_fma(d, c, 0x1.8p52 - z);
         const u64 p = __builtin_bit_cast(u64, exp2(f));
         const unsigned hi = (unsigned)(p >> 32) + (((unsigned)__builtin_bit_cast(u64, z) + (unsigned)frac) << 20);
@@ -134,7 +135,7 @@ struct Weights {
     }
     // The weight itself, however small.
     __device__ __forceinline__ double real(float x) const {
-        const double t = __builtin_fmax(((double)__builtin_fminf(x, 0x1.fffffep+127f) - max) * c, -4096.);
+        const double t = __builtin_fmin(__builtin_fmax(((double)x - max) * c, -4096.), 0.);
         return __builtin_amdgcn_ldexp(exp2(t - __builtin_rint(t)), (int)__builtin_rint(t));
     }
     __device__ __forceinline__ double one() const { return __builtin_amdgcn_ldexp(1., frac); }

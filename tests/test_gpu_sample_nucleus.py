@@ -2,8 +2,10 @@
 the numpy oracle in 64 bits."""
 import numpy as np
 import pytest
+import torch
 
-from test_gpu_sample import _check
+from block_helpers import TYPES, values
+from test_gpu_sample import _check, _sample
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +50,29 @@ def test_flat_and_steep_rows(gpu, rng, cols):
     p = np.tile([1e-6, 0.3, 0.9, 1 - 2.0 ** -24], 11)
     _check(gpu, x, "f32", rng.random(len(T)), T=T, p=p)
     _check(gpu, x, "f32", rng.random(len(T)), T=T, p=p, k=rng.integers(1, cols, len(T)), m=p * 0.01)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cols", [700, 3000, 20001, 40000])
+def test_masked_places(gpu, rng, cols, t):
+    """NaN and infinities among the logits, at temperatures up to infinity: none of a nucleus's mass."""
+    rows = 60
+    x = values(torch.as_tensor(rng.standard_normal((rows, cols)) * 2).to(TYPES[t][1]))
+    for r in range(rows):
+        x[r, rng.integers(0, cols, cols // (2 + r % 5))] = (np.nan, -np.inf)[r % 2]
+    T = np.tile(np.array([0.5, 1.0, 30.0, 1e30, np.inf]), rows // 5)
+    p = rng.random(rows)
+    _check(gpu, x, t, rng.random(rows), T=T, p=p)
+    _check(gpu, x, t, rng.random(rows), T=T, p=p, k=np.full(rows, cols // 2), m=np.full(rows, 0.1))
+
+
+@pytest.mark.parametrize("cols", [4, 700, 40000])
+def test_largest_value_beside_infinity(gpu, cols):
+    """Finite logits have no weight beside an infinite one, the largest fp32 neither."""
+    x = np.full((5, cols), float(torch.finfo(torch.float32).max))
+    x[:, cols // 2] = np.inf
+    off = np.ones(5)
+    for T in (0.5, 1.0, np.inf):
+        for p in (off, 0.5 * off):
+            tok, prob = _sample(gpu, x, "f32", np.linspace(0, 0.99, 5), T=T * off, p=p)
+            assert (tok == cols // 2).all() and (prob == 1).all()
