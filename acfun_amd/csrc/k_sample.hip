@@ -462,7 +462,7 @@ struct Draw {
         });
         __syncthreads();
         const u64 total = block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{}), target = target_of(total);
-        if (target == 0) {                      // u = 0: the first kept, however small its weight
+        if (__builtin_expect(target == 0, 0)) { // u = 0: the first kept, however small its weight
             u64 first = ~0ull;
             each_listed(n, [&](float x, int i) {
                 const u64 at = (u64)(unsigned)i << 32 | __float_as_uint(x);
@@ -525,8 +525,8 @@ struct Draw {
     }
     // Draws from the tokens i0 to i1 not below the cut, those before them having the mass
     // `before` of all tokens' `total` (0: it is that of these).  `runs`: sm.part has the masses of
-    // the waves' runs.
-    __device__ __forceinline__ void from_row(int i0, int i1, u64 cut, u64 before, u64 total, bool runs) const {
+    // the waves' runs.  k: the row's top_k, which the cut does not hold where fewer tokens have a bin.
+    __device__ __forceinline__ void from_row(int i0, int i1, u64 cut, u64 before, u64 total, bool runs, int k) const {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         u64 target = total ? target_of(total) : 1;
         // a run to each wave, then a part of the run that the target falls in
@@ -549,7 +549,16 @@ struct Draw {
             i1 = i0 + per < i1 ? i0 + per : i1;
             if (per == kWaveLoad) break;
         }
-        if (target == 0) {                      // u = 0: the first kept, however small its weight
+        if (__builtin_expect(target == 0, 0)) { // u = 0: the first kept, however small its weight
+            if (k > 0) {                        // (so also among those of the first k without a bin)
+                unsigned binned = 0;
+                all([&](float x, int) { binned += w.bin(x) < (unsigned)kBins; });
+                binned = same(block_all(binned, sm, Add{}));
+                if (binned < (unsigned)k) {
+                    const u64 last = cut_by_digits<false>(kBins, (u64)k, binned);
+                    cut = last > cut ? last : cut;
+                }
+            }
             const Cut c(cut);
             int first = row.cols;
             all([&](float x, int i) {
@@ -583,7 +592,7 @@ struct Draw {
     __device__ __forceinline__ Plan plan(int k, float p, bool by_count) const {
         const int t = threadIdx.x;
         Plan l{by_count, true, false, 0, (u64)k, 0};
-        if (by_count) {                         // (fewer tokens than k that weigh anything: no limit)
+        if (by_count) {                         // (fewer than k tokens with a bin: no limit on what weighs anything)
             l.cut = find_bin(sm.count, l.need, sm);
         } else if (p < 1.f) {
             l.need = same(share(p, block_all(sm.mass[2 * t] + sm.mass[2 * t + 1], sm, Add{})));
@@ -803,7 +812,7 @@ struct Draw {
             if (runs) add_list((int)n, cut, 0, run_of(0, row.cols), sm.part);
             break;
         }
-        from_row(0, row.cols, cut, 0, 0, runs);
+        from_row(0, row.cols, cut, 0, 0, runs, k);
     }
 };
 
@@ -1010,7 +1019,7 @@ __global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
     const int s = __ffsll(past) - 1;
     const u64 before = s ? from_lane(upto, s - 1) : 0;
     const int i0 = s * p.per;
-    d.from_row(i0, i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols, cut, before, total, false);
+    d.from_row(i0, i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols, cut, before, total, false, ask.k);
 }
 
 template <class T>
