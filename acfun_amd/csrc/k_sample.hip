@@ -5,8 +5,11 @@
 //   w_i >= m.  The token is the first in order of index with sum_{j <= i} w_j > u sum w.
 //
 // Weights are 64-bit integers, multiples of 2^-f with f so that a row's sum fits (45 for
-// 2^17 columns), from an exponential in 64 bits: sums do not depend on their order,
-// and the token is the one that real numbers give but for u within about 2^-f of a border.
+// 2^17 columns, 48 at most), from an exponential in 64 bits: sums do not depend on their order.
+// Half a step of each weight and the exponential's 2^-39.8 of it leave a row's shares, and
+// with them the borders that u and a nucleus are compared with, off by cols 2^-(f+1) + 2^-38.8 at
+// most: 2^-28.9 for 2^17 columns, 2^-24.9 for 2^19 and more.  Past 2^19 columns f is taken from the row's
+// own sum, in a pass of its own (1 x 2^20 fp32 with a nucleus 59 us, 50 without it).
 // No row is sorted.  The kept tokens are those not below one of them, the cut, in the
 // order; it lies in a bin of a histogram over x whose tokens alone are put in order.  Bins are
 // even in x / T, 59 to a factor of e, so that most rows spread over many.  A top-k's
@@ -518,6 +521,11 @@ struct Draw {
         });
         return wave_all(mass, Add{});
     }
+    // The mass of all tokens i0 to i1.
+    __device__ __forceinline__ u64 mass_of(int i0, int i1) const {
+        const u64 mass = kept_mass(i0, i1, kNoCut, threadIdx.x, NT);
+        return block_all((threadIdx.x & 63) == 0 ? mass : 0, sm, Add{});
+    }
     // A wave's run of the tokens i0 to i1: whole loads of a wave.
     static constexpr int kWaveLoad = 64 * Row<T>::V;
     static __device__ __forceinline__ int run_of(int i0, int i1) {
@@ -849,8 +857,15 @@ __device__ __forceinline__ void settle(const SampleArgs& a, int r, const Row<T>&
 }
 __device__ __forceinline__ bool settled(float top, const Ask& ask) { return !(top > -__builtin_inff()) || !(ask.T > 0.f); }
 
-// A workgroup to a row, which it reads three to five times.
-template <class T, int NT>
+// f for a row whose `cols` weights have the sum `total` in steps of 2^-frac, each off by half a step: up
+// to kSampleFrac, while the sum stays below 2^62.
+__device__ __forceinline__ int wide_frac(int frac, int cols, u64 total) {
+    const int more = __builtin_clzll(total + (unsigned)cols) - 2;
+    return frac + more < kSampleFrac ? frac + (more > 0 ? more : 0) : kSampleFrac;
+}
+
+// A workgroup to a row, which it reads three to five times (WIDE: once more).
+template <class T, int NT, bool WIDE = false>
 __global__ __launch_bounds__(NT) void k_sample(SampleArgs a, int frac) {
     __shared__ Shared<NT> sm;
     const int r = blockIdx.x;
@@ -861,6 +876,10 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a, int frac) {
         settle(a, r, row, top, 0, a.cols, sm);
         return;
     }
+    if constexpr (WIDE) {
+        const Draw<T, NT> d{row, Weights(top, ask.T, frac, 2 * NT), sm, nullptr, nullptr, 0.f, 0.f};
+        frac = wide_frac(frac, a.cols, d.mass_of(0, a.cols));
+    }
     const Draw<T, NT> d{row, Weights(top, ask.T, frac, 2 * NT), sm, a.token + r, a.prob ? a.prob + r : nullptr, ask.u,
                         ask.m};
     d.from_whole(ask.k, ask.p);
@@ -868,7 +887,7 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a, int frac) {
 
 // ---------------------------------------------------------------- few long rows
 // A row's `parts` workgroups have `per` of its tokens each, in four launches: the largest,
-// the histogram, the list, the draw.
+// the histogram, the list, the draw; and, for wide rows, the sum after the largest.
 struct Split {
     SampleArgs a;
     int frac, parts, per;
@@ -877,13 +896,13 @@ struct Split {
 constexpr int NS = 1024;                        // threads
 struct SplitRow {
     u64 mass[Shared<NS>::kBins], list[Shared<NS>::kList];
-    u64 kept[kSampleParts];
+    u64 kept[kSampleParts], sum[kSampleParts];
     float top[kSampleParts];
     unsigned count[Shared<NS>::kBins];
     unsigned n;
     Plan plan;
 };
-template <class T>
+template <class T, bool WIDE>
 struct Part {
     const int r, part, i0, i1;
     const Row<T> row;
@@ -901,7 +920,10 @@ struct Part {
         return __ffsll(lanes_of(lane < p.parts && ws.top[lane] == top)) - 1;
     }
     __device__ __forceinline__ Draw<T, NS> draw(const Split& p, float top, const Ask& ask, Shared<NS>& sm) const {
-        return {row, Weights(top, ask.T, p.frac, 2 * NS), sm, p.a.token + r, p.a.prob ? p.a.prob + r : nullptr, ask.u,
+        const int lane = threadIdx.x & 63;
+        int frac = p.frac;
+        if constexpr (WIDE) frac = wide_frac(frac, p.a.cols, wave_all(lane < p.parts ? ws.sum[lane] : 0, Add{}));
+        return {row, Weights(top, ask.T, frac, 2 * NS), sm, p.a.token + r, p.a.prob ? p.a.prob + r : nullptr, ask.u,
                 ask.m};
     }
 };
@@ -913,7 +935,7 @@ __device__ __forceinline__ bool plain(float top, const Ask& ask) {
 template <class T>
 __global__ __launch_bounds__(NS) void k_sample_first(Split p) {
     __shared__ Shared<NS> sm;
-    const Part<T> q(p);
+    const Part<T, false> q(p);
     for (int i = q.part * NS + threadIdx.x; i < 2 * NS; i += p.parts * NS) q.ws.mass[i] = 0, q.ws.count[i] = 0;
     if (q.part == 0 && threadIdx.x == 0) q.ws.n = 0;
     const float top = largest_of(q.row, q.i0, q.i1, sm);
@@ -921,9 +943,21 @@ __global__ __launch_bounds__(NS) void k_sample_first(Split p) {
 }
 
 template <class T>
+__global__ __launch_bounds__(NS) void k_sample_sum(Split p) {
+    __shared__ Shared<NS> sm;
+    const Part<T, false> q(p);
+    const Ask ask(p.a, q.r);
+    const float top = q.top(p);
+    if (settled(top, ask)) return;
+    const Draw<T, NS> d{q.row, Weights(top, ask.T, p.frac, 2 * NS), sm, nullptr, nullptr, 0.f, 0.f};
+    const u64 mass = d.mass_of(q.i0, q.i1);
+    if (threadIdx.x == 0) q.ws.sum[q.part] = mass;
+}
+
+template <class T, bool WIDE>
 __global__ __launch_bounds__(NS) void k_sample_bins(Split p) {
     __shared__ Shared<NS> sm;
-    const Part<T> q(p);
+    const Part<T, WIDE> q(p);
     const Ask ask(p.a, q.r);
     const float top = q.top(p);
     if (plain(top, ask)) return;
@@ -938,8 +972,8 @@ __global__ __launch_bounds__(NS) void k_sample_bins(Split p) {
 }
 
 // The row's histogram from memory, and its plan.
-template <class T>
-__device__ __forceinline__ Plan plan_of(const Part<T>& q, const Draw<T, NS>& d, const Ask& ask) {
+template <class T, bool WIDE>
+__device__ __forceinline__ Plan plan_of(const Part<T, WIDE>& q, const Draw<T, NS>& d, const Ask& ask) {
     for (int i = threadIdx.x; i < 2 * NS; i += NS) d.sm.count[i] = q.ws.count[i], d.sm.mass[i] = q.ws.mass[i];
     __syncthreads();
     const Plan l = d.plan(ask.k, ask.p, ask.k > 0);
@@ -948,10 +982,10 @@ __device__ __forceinline__ Plan plan_of(const Part<T>& q, const Draw<T, NS>& d, 
 // A top-k of many tokens with a nucleus among them: one workgroup does such a row.
 __device__ __forceinline__ bool hard(const Plan& l, const Ask& ask) { return l.by_count && !l.take && ask.p < 1.f; }
 
-template <class T>
+template <class T, bool WIDE>
 __global__ __launch_bounds__(NS) void k_sample_take(Split p) {
     __shared__ Shared<NS> sm;
-    const Part<T> q(p);
+    const Part<T, WIDE> q(p);
     const Ask ask(p.a, q.r);
     const float top = q.top(p);
     if (settled(top, ask)) return;
@@ -980,11 +1014,11 @@ __global__ __launch_bounds__(NS) void k_sample_take(Split p) {
 }
 
 // A workgroup to a row.
-template <class T>
+template <class T, bool WIDE>
 __global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
     __shared__ Shared<NS> sm;
     __shared__ u64 kept[kSampleParts];
-    const Part<T> q(p);
+    const Part<T, WIDE> q(p);
     const Ask ask(p.a, q.r);
     const float top = q.top(p);
     if (settled(top, ask)) {
@@ -1022,22 +1056,22 @@ __global__ __launch_bounds__(NS) void k_sample_draw(Split p) {
     d.from_row(i0, i0 + p.per < p.a.cols ? i0 + p.per : p.a.cols, cut, before, total, false, ask.k);
 }
 
-template <class T>
+template <class T, bool WIDE>
 bool launch_split(const Split& p, bool cuts, hipStream_t s) {
     const dim3 grid((unsigned)p.parts, (unsigned)p.a.rows), block(NS);
     ACFUN_LAUNCH("k_sample_first", (k_sample_first<T>), grid, block, 0, s, p);
-    if (cuts) ACFUN_LAUNCH("k_sample_bins", (k_sample_bins<T>), grid, block, 0, s, p);
-    ACFUN_LAUNCH("k_sample_take", (k_sample_take<T>), grid, block, 0, s, p);
-    ACFUN_LAUNCH("k_sample_draw", (k_sample_draw<T>), dim3(1, (unsigned)p.a.rows), block, 0, s, p);
+    if (WIDE) ACFUN_LAUNCH("k_sample_sum", (k_sample_sum<T>), grid, block, 0, s, p);
+    if (cuts) ACFUN_LAUNCH("k_sample_bins", (k_sample_bins<T, WIDE>), grid, block, 0, s, p);
+    ACFUN_LAUNCH("k_sample_take", (k_sample_take<T, WIDE>), grid, block, 0, s, p);
+    ACFUN_LAUNCH("k_sample_draw", (k_sample_draw<T, WIDE>), dim3(1, (unsigned)p.a.rows), block, 0, s, p);
     return check_launch("k_sample_draw");
 }
 
 }  // namespace
 
 bool sample_rows(const SampleArgs& a, int type, hipStream_t s) {
-    int bits = 0;
-    while ((1 << bits) < a.cols) ++bits;
-    const int frac = 62 - bits < 48 ? 62 - bits : 48;
+    const int frac = sample_frac(a.cols);
+    const bool wide = a.cols > kSampleEven;
     const SamplePlan plan = sample_plan(a.rows, a.cols, num_cus());
     bool split = plan.parts > 1;
     if (split) {
@@ -1050,14 +1084,18 @@ bool sample_rows(const SampleArgs& a, int type, hipStream_t s) {
         using T = decltype(t);
         if (split) {
             Scratch ws((size_t)a.rows * sizeof(SplitRow), s);
-            return ws.p && launch_split<T>({a, frac, plan.parts, plan.per, ws.as<char>()}, a.top_k || a.top_p, s);
+            const Split p{a, frac, plan.parts, plan.per, ws.as<char>()};
+            const bool cuts = a.top_k || a.top_p;
+            return ws.p && (wide ? launch_split<T, true>(p, cuts, s) : launch_split<T, false>(p, cuts, s));
         }
         if (plan.threads == 256)
             ACFUN_LAUNCH("k_sample", (k_sample<T, 256>), dim3(a.rows), dim3(256), 0, s, a, frac);
         else if (plan.threads == 512)
             ACFUN_LAUNCH("k_sample", (k_sample<T, 512>), dim3(a.rows), dim3(512), 0, s, a, frac);
-        else
+        else if (!wide)
             ACFUN_LAUNCH("k_sample", (k_sample<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a, frac);
+        else
+            ACFUN_LAUNCH("k_sample", (k_sample<T, 1024, true>), dim3(a.rows), dim3(1024), 0, s, a, frac);
         return check_launch("k_sample");
     });
 }

@@ -121,6 +121,15 @@ constexpr bool q8_rows_one(int M, int K) { return M <= 16 && M * (((long long)K 
 // A workgroup of `threads` to a row, or `parts` of 1024 with `per` columns each (whole
 // 1024s, which are two waves' loads).
 constexpr int kSampleMaxCols = 1 << 24, kSampleParts = 32;
+// A row's sum of weights is below 2^63 in steps of 2^-f.  With f for the most that `cols` weights can
+// have, half a step for each is 2^-25 of the largest weight up to this many; wider rows have f for what
+// theirs have.
+constexpr int kSampleFrac = 48, kSampleEven = 1 << 19;
+constexpr int sample_frac(int cols) {
+    int bits = 0;
+    while ((1 << bits) < cols) ++bits;
+    return 62 - bits < kSampleFrac ? 62 - bits : kSampleFrac;
+}
 constexpr bool sample_fits(int rows) { return launch_fits(rows, 1024); }
 struct SamplePlan { int parts, per, threads; };
 // Parts from 24,576 columns on while a row has 2,048 columns for each row of the call.

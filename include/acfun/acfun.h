@@ -389,9 +389,11 @@ void acfun_fc_gated_q8(const float* input, int N, int Cin, const int8_t* gate, c
  * NaN) and 1 - 2^-24.  token [rows] gets the index, -1 for a row with nothing to draw,
  * and prob [rows] (NULL: not wanted) the probability it was drawn with, 0 for -1.
  * Sums of weights are in integers of 64 bits and the same in any order, so that a row's
- * token does not depend on the other rows or on the launch.  Few long rows take four
- * launches and a workspace from the library's pool; others, and every call on a stream that
- * is being captured into a graph, one launch without temporaries. */
+ * token does not depend on the other rows or on the launch.  Weights' roundings leave the
+ * parts of a sum that u and top_p are compared with off by at most 2^-28.9 up to 2^17
+ * columns, 2^-24.9 past 2^19.  Few long rows take four launches (past 2^19 columns five) and
+ * a workspace from the library's pool; others, and every call on a stream that is being
+ * captured into a graph, one launch without temporaries. */
 int acfun_dev_sample(const void* logits, int type, int rows, int cols, int ld, const float* temperature,
                      const int* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
                      float* prob, void* stream);
