@@ -2,7 +2,6 @@
 codes, the library's byte layout), the norms around a block, activations and the draw
 of a token.  Written from the definitions in include/acfun/acfun.h."""
 import numpy as np
-from scipy.special import erfc
 
 LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
 
@@ -119,6 +118,7 @@ def act(v, kind):
         if kind == 2:
             return v / (1 + np.exp(-v))
         if kind == 3:
+            from scipy.special import erfc                   # (what uses no GELU needs no scipy)
             return 0.5 * v * erfc(-v / np.sqrt(2))
         if kind == 4:
             return v / (1 + np.exp(-2 * np.sqrt(2 / np.pi) * (v + 0.044715 * v ** 3)))
