@@ -1,11 +1,13 @@
 // k_q8.hip -- the Q8 quantizer and its inverse (layout and rounding: q8.hpp).
 //
-// Memory bounds them.  A row's scale is known once all of it has been read, so a
-// workgroup keeps its rows in LDS (columns: in registers) between the two and reads them
-// once; past what those hold the end of a row is read again.  Measured, a copy of 4 GiB
-// at 4.9 TB/s beside them: 4096 x 4096 bf16 10.8 us with the input in the caches (4.7 TB/s), 17.0
-// after other work, and 9.9 back; weights fp32 [4096][8192] 54.7 us (3.1 TB/s), 28.0
-// back (6.0 TB/s, the codes from the caches); 8192 x 8192 bf16 46 us (4.4 TB/s).
+// A row's scale is known once all of it has been read, so a workgroup keeps its rows in LDS
+// (columns: in registers) between the two and reads them once; past what those hold the end
+// of a row is read again.  4096 x 4096 bf16 takes 10.8 us with the input in the caches, 16 to 17
+// after other work, 8192 x 8192 46.  A copy's 5.55 TB/s would be 9.1 for the first; the codes' loop
+// has some 100 instructions to a turn, 8 turns to a wave, 8 waves to a SIMD, which is 10.7,
+// three quarters of it in turns without values (below).  Weights wait for whole columns: fp32
+// [4096][8192] 53 to 55 us (3.1 TB/s).  Reading back is bound by memory: 9.9 us, and 26.6
+// to 28.0 for the weights (6.0 TB/s, the codes from the caches).
 #include <type_traits>
 
 #include "mm.hpp"
@@ -75,6 +77,8 @@ __global__ __launch_bounds__(kQ8RowThreads) void k_q8_quant(const T* __restrict_
     for (int i = 0; i < W; ++i) top = umax(top, tops[i][r]);
     const Q8Scale sc(top);
     if (w == 0 && p0 == 0) scales[row] = sc.s;
+    // A turn for every 64 k of the row, though a step has 16 P of them: the turns from `steps` on,
+    // 6 of a wave's 8 for R = 4 and K = 4096, find codes of zeros and store nothing.
 #pragma unroll 1
     for (int i = 0; w + i * W < kt; ++i) {
         const int step = w + i * W, p = P * step + p0;

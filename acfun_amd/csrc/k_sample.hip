@@ -8,8 +8,9 @@
 // 2^17 columns, 48 at most), from an exponential in 64 bits: sums do not depend on their order.
 // Half a step of each weight and the exponential's 2^-39.8 of it leave a row's shares, and
 // with them the borders that u and a nucleus are compared with, off by cols 2^-(f+1) + 2^-38.8 at
-// most: 2^-28.9 for 2^17 columns, 2^-24.9 for 2^19 and more.  Past 2^19 columns f is taken from the row's
-// own sum, in a pass of its own (1 x 2^20 fp32 with a nucleus 59 us, 50 without it).
+// most: 2^-28.9 for 2^17 columns, 2^-24.9 for 2^19 and more.  Past 2^19 columns f is taken
+// from the row's own sum, in a pass of its own (1 x 2^20 fp32 with a nucleus 59 us, 50 without
+// it; where the border's bin has more tokens than a list, one workgroup does the row again: 1.8 ms).
 // No row is sorted.  The kept tokens are those not below one of them, the cut, in the
 // order; it lies in a bin of a histogram over x whose tokens alone are put in order.  Bins are
 // even in x / T, 59 to a factor of e, so that most rows spread over many.  A top-k's
@@ -18,7 +19,8 @@
 //
 // A row is read three to five times from the caches, and a few rows wait for what follows one
 // another: 64 x 32003 bf16 takes 7.5 us for the largest, 15.7 with a temperature, 23 with a top-k,
-// 33 with a nucleus, 27 with all; 64 x 1000 fp32 3.7, 4.8, 8, 12 and 13.  Many rows are bound by the
+// 33 with a nucleus, 27 with all; 64 x 1000 fp32 3.7, 4.8, 8, 12 and 13.  A captured call has one
+// workgroup to any row: 1 x 131072 fp32 with all settings 40 us, 24 in parts.  Many rows are bound by the
 // instructions of a weight, the exponential in 64 bits above all: 512 x 131072 fp32 with a
 // nucleus takes 207 us, half of it the one pass with weights; the first, from memory, 46.
 #include <type_traits>

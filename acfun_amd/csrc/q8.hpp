@@ -111,9 +111,10 @@ __device__ __forceinline__ int2 bytes8(const unsigned (&c)[8]) {
     return {low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7])};
 }
 
-// Activations, as in the header.  exp by the hardware's 2^x: one
-// step of its argument is |v| / 2^24 of the result, which bf16 and fp16 do not show;
-// EXACT (fp32 results) adds what the argument's rounding lost.  NaN stays NaN.
+// Activations, as in the header.  exp by the hardware's 2^x, off by a step, 2^-23; half a
+// step of its argument is |v| 2^-24 of the result, and the reciprocal is off by a step: 2^-17
+// in all for |v| up to 88, beside half a step of bf16 and fp16, 2^-9 and 2^-12 of a value at
+// least.  EXACT (fp32 results) adds what the argument's rounding lost, and divides.  NaN stays NaN.
 template <bool EXACT>
 __device__ __forceinline__ float exp_of(float v) {
     constexpr float L = 0x1.715476p+0f, l = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;  // log2 e = L + l

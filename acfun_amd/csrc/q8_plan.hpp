@@ -21,7 +21,8 @@ constexpr int kQ8RowThreads = 512;
 constexpr long long q8_row_groups(int rows, int R) { return q8_row_tiles(rows) * (16 / R); }
 // Two rows while a CU has one workgroup of them at most, four past that.  Measured, us, bf16,
 // K of 4096: 16 rows 2.8 and 3.9 with four (8.7 with 16), 512 rows 3.6 and 4.4, 1024
-// rows 5.8 and 4.9, 4096 rows 12.8 and 10.8 (15.1 with 16).
+// rows 5.8 and 4.9, 4096 rows 12.8 and 10.8 (15.1 with 16); the kernel's turns without values, of
+// which two rows have twice as many, are in these.
 constexpr int q8_rows_of(int rows, int cus) { return rows <= 2 * cus ? 2 : 4; }
 // The steps that a wave keeps in LDS: a power of two, 64 KB at most.
 constexpr int q8_row_steps(int K, int R, size_t elem) {
@@ -113,8 +114,9 @@ constexpr bool q8_rows_fit(int M, int N, int K, bool gated) {
     return q8_few_sums(1, 1, 8, gated ? 2 : 1) + q8_rows_lds(M, K) <= kLds && q8_mm_fits(M, N, K, Q8_FEW16, gated);
 }
 // It is taken up to two pieces of a row and 512 k for each of its 8 waves, which take 0.6
-// us and 0.8 for each; a launch of the quantizer takes 2.8.  Measured, us, K and N of 4096,
-// in one and in two: 1 row 6.6 and 8.1, 2 rows 7.4 and 8.1, 4 rows 8.7 and 8.1, 16 rows 19 and 8.2.
+// us and 0.8 for each; a launch of the quantizer takes 2.8, its turns without values among
+// them.  Measured, us, K and N of 4096, in one and in two: 1 row 6.6 and 8.1, 2 rows 7.4 and
+// 8.1, 4 rows 8.7 and 8.1, 16 rows 19 and 8.2.
 constexpr bool q8_rows_one(int M, int K) { return M <= 16 && M * (((long long)K + 511) / 512) <= 16; }
 
 // ---------------------------------------------------------------- sampling
@@ -135,8 +137,8 @@ struct SamplePlan { int parts, per, threads; };
 // Parts from 24,576 columns on while a row has 2,048 columns for each row of the call.
 // Measured, us, one workgroup (in a graph) and parts: mixed settings bf16 1 x 32768 18 and
 // 20, 1 x 131072 36 and 20, 16 x 65536 45 and 31, 64 x 131072 101 and 61; a nucleus fp32 1 x 32768
-// 28 and 23, 32 x 65536 47 and 41; all settings on fp32 1 x 32768 23 and 23, 32 x 65536 31 and
-// 37, 64 x 65536 32 and 41, 128 x 131072 52 and 68.
+// 28 and 23, 32 x 65536 47 and 41; all settings on fp32 1 x 32768 23 and 23, 1 x 131072 40 and 24,
+// 32 x 65536 31 and 37, 64 x 65536 32 and 41, 128 x 131072 52 and 68.
 inline SamplePlan sample_plan(int rows, int cols, int cus) {
     if (cols < 24576 || (long long)rows * 2048 > cols)
         return {1, cols, cols <= 1024 ? 256 : cols <= 8192 ? 512 : 1024};
